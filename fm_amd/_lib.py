@@ -1,4 +1,4 @@
-"""ctypes binding of libfmscan_hip.so (interface: include/fmscan.h).
+"""ctypes binding of libfmscan_hip.so (interface: include/fmscan.h, include/fmselective.h).
 
 There is no other implementation behind these calls: if the library cannot
 be loaded the import of `fm_amd.scan.fm_scan` fails, and tensors that are not
@@ -11,7 +11,7 @@ from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint, c_void_p
 
 from . import build as _build
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 FLAG_PLAIN = 0x1
@@ -19,6 +19,9 @@ FLAG_WAVES_SHIFT = 8
 FLAG_BLOCKS_SHIFT = 12
 FLAG_DEPTH_SHIFT = 16
 FLAG_SEGMENTS_SHIFT = 20
+# include/fmselective.h
+SELECTIVE_SOFTPLUS, SELECTIVE_SILU, SELECTIVE_SLOTS_64 = 0x1, 0x2, 0x4
+SELECTIVE_NARROW_WEIGHT, SELECTIVE_NARROW_BIAS, SELECTIVE_NARROW_SKIP = 0x10, 0x20, 0x40
 
 _lib = None
 
@@ -141,6 +144,17 @@ def load() -> ctypes.CDLL:
     lib.fmscan_readout_backward.argtypes = [c_void_p] * 8 + dims + [c_int, c_void_p]
     lib.fmscan_swap_last_two.restype = c_int
     lib.fmscan_swap_last_two.argtypes = [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]
+    lib.fmselective_conv_forward.restype = c_int
+    lib.fmselective_conv_forward.argtypes = ([c_void_p, c_int64, c_int64] + [c_void_p] * 6 + [c_int64] * 4
+                                             + [c_int, c_uint, c_void_p])
+    lib.fmselective_conv_workspace_bytes.restype = c_size_t
+    lib.fmselective_conv_workspace_bytes.argtypes = [c_int64] * 4 + [c_int]
+    lib.fmselective_conv_backward.restype = c_int
+    lib.fmselective_conv_backward.argtypes = ([c_void_p, c_int64, c_int64] * 2 + [c_void_p] * 9 + [c_int64] * 4
+                                              + [c_int, c_uint, c_void_p, c_size_t, c_void_p])
+    lib.fmselective_conv_step.restype = c_int
+    lib.fmselective_conv_step.argtypes = ([c_void_p, c_int64] + [c_void_p] * 6 + [c_int64] * 4
+                                          + [c_int, c_uint, c_void_p])
     got = lib.fmscan_abi_version()
     if got != ABI_VERSION:
         raise RuntimeError(f"libfmscan_hip.so has ABI version {got}, this package needs {ABI_VERSION}; "

@@ -1,0 +1,261 @@
+// Kernels of the short depthwise convolution along time: forward, backward, one token.
+//
+// All three are bound by memory: a row is read once and written once, W <= 4 multiply-adds an element.
+#pragma once
+
+#include "fmselective_device.h"
+
+namespace fmselective {
+
+// W - 1 values before chunk position t0 of a row: the row's own where t0 > 0 (a chunk has at least 4 elements and
+// chunks start at multiples of that, so t0 >= 4), else the carried state's, else zeros.
+template <typename T, int W>
+__device__ __forceinline__ void values_before(const T* __restrict__ row, int64_t t0, int64_t len,
+                                              const T* __restrict__ state, float (&f)[W - 1]) {
+    if (t0 > 0) {
+        if (t0 > len) {  // nothing of this chunk counts
+#pragma unroll
+            for (int i = 0; i < W - 1; ++i) f[i] = 0.0f;
+        } else if constexpr (sizeof(T) == 4) {
+            const u32x4 v = fmscan::load16<T, false, false>(row + t0 - 4);
+#pragma unroll
+            for (int i = 0; i < W - 1; ++i) f[i] = u2f(v[i + 5 - W]);
+        } else {
+            typedef uint32_t u32x2_at2 __attribute__((ext_vector_type(2), aligned(2)));
+            const u32x2_at2 v = *reinterpret_cast<const u32x2_at2*>(row + t0 - 4);
+            u32x4 wide = {v.x, v.y, 0u, 0u};
+            float four[8];
+            Elem<T>::unpack(wide, four);
+#pragma unroll
+            for (int i = 0; i < W - 1; ++i) f[i] = four[i + 5 - W];
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) f[i] = state ? Elem<T>::widen(state[i]) : 0.0f;
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void conv_taps(const void* weight, const void* bias, int64_t d, unsigned flags,
+                                          float (&w)[W], float& b) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j] = param<T>(weight, d * W + j, flags & FMSELECTIVE_NARROW_WEIGHT);
+    b = bias ? param<T>(bias, d, flags & FMSELECTIVE_NARROW_BIAS) : 0.0f;
+}
+
+struct ConvRows {
+    int64_t batch_stride, channel_stride, L;
+    int32_t rows, D;
+    uint32_t tiles;         // blocks a row takes (1 where a block takes whole rows)
+    uint32_t rows_per_block;
+    uint32_t chunks;        // of a row
+    uint32_t magic;         // ceil(2^16 / chunks), for rows_per_block > 1
+};
+
+// One chunk of 16 bytes a thread; the W - 1 values before it are a second, 8-byte load that the L1 answers.
+// Short rows are packed: a block takes as many whole rows as it has threads for.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void conv_forward_kernel(const T* __restrict__ inputs, const void* __restrict__ weight,
+                                                           const void* __restrict__ bias, const T* __restrict__ initial,
+                                                           const int32_t* __restrict__ lengths, T* __restrict__ out,
+                                                           T* __restrict__ final_state, ConvRows g, unsigned flags) {
+    constexpr int E = Elem<T>::E;
+    uint32_t row, chunk;
+    if (g.rows_per_block > 1) {
+        const uint32_t r = (threadIdx.x * g.magic) >> 16;
+        if (r >= g.rows_per_block) return;
+        row = blockIdx.x * g.rows_per_block + r;
+        chunk = threadIdx.x - r * g.chunks;
+    } else {
+        row = g.tiles == 1 ? blockIdx.x : blockIdx.x / g.tiles;
+        chunk = (blockIdx.x - row * g.tiles) * blockDim.x + threadIdx.x;
+    }
+    if (row >= (uint32_t)g.rows || chunk >= g.chunks) return;
+    const uint32_t b = row / (uint32_t)g.D, d = row - b * g.D;
+    const int64_t len = row_length(lengths, b, g.L), t0 = (int64_t)chunk * E;
+    const T* x = inputs + b * g.batch_stride + d * g.channel_stride;
+    const T* state = initial ? initial + (int64_t)row * (W - 1) : nullptr;
+    float w[W], bv, f[E], before[W - 1], y[E];
+    load_values<T, E>(x, t0, len, f);
+    values_before<T, W>(x, t0, len, state, before);
+    conv_taps<T, W>(weight, bias, d, flags, w, bv);
+    auto at = [&](int i) { return i < 0 ? before[i + W - 1] : f[i]; };
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        float v = bv;
+#pragma unroll
+        for (int j = 0; j < W; ++j) v = __builtin_fmaf(w[j], at(k - (W - 1) + j), v);
+        if (flags & FMSELECTIVE_SILU) v *= sigmoid(v);
+        y[k] = t0 + k < len ? v : 0.0f;
+    }
+    store_values<T, E>(out + (int64_t)row * g.L, t0, g.L, y);
+    if (final_state && chunk == 0) {
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i) {
+            const int64_t p = len - (W - 1) + i;
+            final_state[(int64_t)row * (W - 1) + i] = p >= 0 ? x[p] : (state ? state[p + W - 1] : (T)0.0f);
+        }
+    }
+}
+
+struct ConvBack {
+    int64_t batch_stride, channel_stride, grad_batch_stride, grad_channel_stride, L;
+    int32_t rows, D;
+    int32_t lanes_log2;   // lanes a row takes in a wave
+    int32_t tiles;        // of 64 chunks, where lanes_log2 is 6; else 1
+    int32_t segments, seg_tiles;
+};
+
+// d pre of one position: the gradient of the sum under the activation
+__device__ __forceinline__ float conv_dpre(float pre, float dy, bool silu) {
+    return silu ? dy * silu_slope(pre, sigmoid(pre)) : dy;
+}
+
+// A wave walks a row (or a segment of a long one) from its end to its start, one chunk a lane: the gradient of
+// the sum before the activation is computed once an element, the W - 1 of them that a lane needs from beyond its
+// chunk come from the next lane, and the last lane's from the tile before (lane 0's, kept). The gradients of
+// weight and bias are summed over the whole walk in registers and across the lanes once. Rows of fewer than
+// 64 chunks share a wave, 2^lanes_log2 lanes each.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void conv_backward_kernel(const T* __restrict__ inputs, const T* __restrict__ out_grad,
+                                                            const void* __restrict__ weight, const void* __restrict__ bias,
+                                                            const T* __restrict__ initial, const T* __restrict__ final_grad,
+                                                            const int32_t* __restrict__ lengths, T* __restrict__ inputs_grad,
+                                                            T* __restrict__ initial_grad, float* __restrict__ weight_part,
+                                                            float* __restrict__ bias_part, ConvBack g, unsigned flags) {
+    constexpr int E = Elem<T>::E, H = W - 1;
+    const int lane = threadIdx.x & 63;
+    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lanes = 1 << g.lanes_log2, c = lane & (lanes - 1);
+    const int64_t slot = (wave << (6 - g.lanes_log2)) + (lane >> g.lanes_log2);  // row, or segment of a row
+    const int64_t want_row = g.segments == 1 ? slot : slot / g.segments;
+    const int32_t seg = g.segments == 1 ? 0 : (int32_t)(slot - want_row * g.segments);
+    const bool live = want_row < g.rows;
+    const int32_t row = live ? (int32_t)want_row : g.rows - 1;
+    const int32_t b = row / g.D, d = row - b * g.D;
+    const int64_t L = live ? g.L : 0;  // a lane without a row loads and stores nothing
+    const int64_t len = live ? row_length(lengths, b, g.L) : 0;
+    const bool silu = flags & FMSELECTIVE_SILU;
+    const T* x = inputs + b * g.batch_stride + d * g.channel_stride;
+    const T* dy = out_grad + b * g.grad_batch_stride + d * g.grad_channel_stride;
+    const T* state = initial ? initial + (int64_t)row * H : nullptr;
+    const T* fg = final_grad ? final_grad + (int64_t)row * H : nullptr;
+    float w[W], bv;
+    conv_taps<T, W>(weight, bias, d, flags, w, bv);
+
+    const int32_t lo = seg * g.seg_tiles;
+    const int32_t hi = lo + g.seg_tiles < g.tiles ? lo + g.seg_tiles : g.tiles;
+    const int64_t tile = (int64_t)lanes * E;
+    float carry[H];  // d pre of the H positions behind the tile at work
+    {
+        const int64_t end = hi * tile;
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            carry[i] = 0.0f;
+            if (end + i < len) {  // the segment behind is another wave's: its first positions again
+                float pre = bv;
+#pragma unroll
+                for (int j = 0; j < W; ++j) pre = __builtin_fmaf(w[j], Elem<T>::widen(x[end + i - H + j]), pre);
+                carry[i] = conv_dpre(pre, Elem<T>::widen(dy[end + i]), silu);
+            }
+        }
+    }
+    float dw[W], db = 0.0f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) dw[j] = 0.0f;
+    float dpre[E + H];
+#pragma unroll
+    for (int k = 0; k < E + H; ++k) dpre[k] = 0.0f;
+    for (int32_t i = hi - 1; i >= lo; --i) {
+        const int64_t t0 = i * tile + (int64_t)c * E;
+        float f[E], gy[E], before[H], dx[E];
+        load_values<T, E>(x, t0, len, f);
+        load_values<T, E>(dy, t0, len, gy);
+        values_before<T, W>(x, t0, len, state, before);
+        auto at = [&](int p) { return p < 0 ? before[p + H] : f[p]; };
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            float pre = bv;
+#pragma unroll
+            for (int j = 0; j < W; ++j) pre = __builtin_fmaf(w[j], at(k - H + j), pre);
+            const bool in = t0 + k < len;
+            dpre[k] = in ? conv_dpre(pre, gy[k], silu) : 0.0f;
+            // (a position that does not count adds nothing, whatever stands before it)
+#pragma unroll
+            for (int j = 0; j < W; ++j) dw[j] = __builtin_fmaf(dpre[k], in ? at(k - H + j) : 0.0f, dw[j]);
+            db += dpre[k];
+        }
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+            const float next = fmscan::dpp<fmscan::kWaveShl1>(0.0f, dpre[k]);
+            dpre[E + k] = c == lanes - 1 ? carry[k] : next;
+            carry[k] = fmscan::lane_value(dpre[k], 0);  // read by rows that fill the wave alone
+        }
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < W; ++j) v = __builtin_fmaf(w[j], dpre[k + H - j], v);
+            const int64_t p = t0 + k - (len - H);  // place in the final state
+            if (fg && p >= 0 && p < H && t0 + k < len) v += Elem<T>::widen(fg[p]);
+            dx[k] = t0 + k < len ? v : 0.0f;
+        }
+        store_values<T, E>(inputs_grad + (int64_t)row * g.L, t0, L, dx);
+    }
+    if (initial_grad && live && seg == 0 && c == 0) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            float v = 0.0f;
+            if (len > 0) {
+#pragma unroll
+                for (int j = 0; j <= i; ++j) v = __builtin_fmaf(w[j], dpre[i - j], v);
+            }
+            if (fg && i >= len) v += Elem<T>::widen(fg[i - len]);
+            initial_grad[(int64_t)row * H + i] = (T)v;
+        }
+    }
+    auto over_lanes = [&](float v) {
+        for (int s = lanes >> 1; s > 0; s >>= 1) v += __shfl_xor(v, s);
+        return v;
+    };
+    const int64_t at = (int64_t)seg * g.rows + row;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        const float v = over_lanes(dw[j]);
+        if (live && c == 0) weight_part[at * W + j] = v;
+    }
+    db = over_lanes(db);
+    if (live && c == 0) bias_part[at] = db;
+}
+
+// One token: a thread a channel of a row. The state moves by one place and takes the new input.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void conv_step_kernel(const T* __restrict__ inputs, int64_t batch_stride, const T* state,
+                                                        T* state_out, const void* __restrict__ weight,
+                                                        const void* __restrict__ bias, const void* __restrict__ slots,
+                                                        T* __restrict__ out, int32_t D, uint32_t tiles, int64_t S,
+                                                        unsigned flags) {
+    const uint32_t b = tiles == 1 ? blockIdx.x : blockIdx.x / tiles;
+    const int64_t d = (int64_t)(blockIdx.x - b * tiles) * blockDim.x + threadIdx.x;
+    const int64_t slot = slot_of_row(slots, flags & FMSELECTIVE_SLOTS_64, (int32_t)b, S);
+    if (d >= D) return;
+    if (slot < 0) {
+        out[(int64_t)b * D + d] = (T)0.0f;
+        return;
+    }
+    const int64_t at = (slot * D + d) * (W - 1);
+    T window[W];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) window[j] = state[at + j];
+    window[W - 1] = inputs[b * batch_stride + d];
+    float w[W], v;
+    conv_taps<T, W>(weight, bias, d, flags, w, v);
+#pragma unroll
+    for (int j = 0; j < W; ++j) v = __builtin_fmaf(w[j], Elem<T>::widen(window[j]), v);
+    if (flags & FMSELECTIVE_SILU) v *= sigmoid(v);
+    out[(int64_t)b * D + d] = (T)v;
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) state_out[at + j] = window[j + 1];
+}
+
+}  // namespace fmselective

@@ -1,0 +1,75 @@
+/*
+ * fmselective.h -- C ABI of libfmscan_hip.so, second part: the operators of a selective state space
+ * layer for AMD MI355X (gfx950), for training, for prompts and for single tokens.
+ *
+ *   short convolution   y[b,d,t] = act(bias[d] + sum_j weight[d,j] x[b,d,t-W+1+j]),  W taps, depthwise
+ *   selective scan      dt = softplus(delta + delta_bias),  h[n] = exp(dt A[d,n]) h[n] + dt u write[n],
+ *                       out = (sum_n read[n] h[n] + skip[d] u) * silu(gate)
+ *   norm                r = inputs + residual,  out = r / sqrt(mean r^2 + eps) * weight, optionally in 8 bits
+ *
+ * The conventions are those of fmscan.h: device pointers on the current GPU, kernels enqueued on `stream`
+ * (a hipStream_t), nothing kept between calls, no memory owned, 0 or an FMSCAN_E_* code or a positive
+ * hipError_t back, the text from fmscan_last_error(). The reference has no counterpart of these operators.
+ *
+ * Sequences are time last. Inputs (B, D, L) may have any batch and channel stride (in elements, >= 0); the
+ * time stride is 1. Outputs are dense. Parameters (weight, bias, skip, delta_bias) are float32 or of the
+ * inputs' element type, one FMSELECTIVE_NARROW_* flag each for the latter.
+ *
+ * lengths (B) int32 or NULL: the steps that count of each row of a padded batch, clamped to [0, L]. Beyond
+ * them inputs are not read, outputs and gradients are zero, and the final state is that after the last
+ * step that counts (the initial state where none does).
+ *
+ * slots (B) int32 or int64, or NULL (row b has slot b, and there are B slots): where in the pool of states a
+ * row of a single-token call has its state. A row whose slot is outside [0, S) is skipped: it gives zeros and
+ * touches no state. Where a slot is named more than once the first row takes it and the later ones are
+ * skipped in the same way.
+ */
+#ifndef FMSELECTIVE_H_
+#define FMSELECTIVE_H_
+
+#include "fmscan.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define FMSELECTIVE_SOFTPLUS        0x1u  /* scan, step: dt = softplus(delta + delta_bias), else the sum itself */
+#define FMSELECTIVE_SILU            0x2u  /* convolution: silu of the sum */
+#define FMSELECTIVE_SLOTS_64        0x4u  /* slots are int64 */
+#define FMSELECTIVE_NARROW_WEIGHT   0x10u /* weight has the inputs' element type */
+#define FMSELECTIVE_NARROW_BIAS     0x20u /* so has bias or delta_bias */
+#define FMSELECTIVE_NARROW_SKIP     0x40u /* so has skip */
+
+/* ---- short convolution --------------------------------------------------------------------------------
+ * W is 2, 3 or 4. bias, initial_state, lengths and final_state may be NULL.
+ *   inputs (B, D, L) strided, weight (D, W), bias (D), initial_state (B, D, W-1): the inputs before the first
+ *   out (B, D, L), final_state (B, D, W-1): the last W-1 inputs that count (out) */
+int fmselective_conv_forward(const void* inputs, int64_t batch_stride, int64_t channel_stride, const void* weight,
+                             const void* bias, const void* initial_state, const int32_t* lengths, void* out,
+                             void* final_state, int64_t B, int64_t D, int64_t L, int64_t W, int dtype,
+                             unsigned flags, void* stream);
+
+/* Bytes of workspace that the backward call needs (its partial sums of the parameters' gradients); 0 where the
+ * sizes are not valid. */
+size_t fmselective_conv_workspace_bytes(int64_t B, int64_t D, int64_t L, int64_t W, int dtype);
+
+/* Gradients. out_grad (B, D, L) strided; final_state_grad (B, D, W-1) or NULL; inputs_grad (B, D, L) dense;
+ * weight_grad (D, W), bias_grad (D) or NULL, of the types of weight and bias; initial_state_grad (B, D, W-1) or
+ * NULL. `bias` is needed for the silu. */
+int fmselective_conv_backward(const void* inputs, int64_t batch_stride, int64_t channel_stride, const void* out_grad,
+                              int64_t grad_batch_stride, int64_t grad_channel_stride, const void* weight,
+                              const void* bias, const void* initial_state, const void* final_state_grad,
+                              const int32_t* lengths, void* inputs_grad, void* weight_grad, void* bias_grad,
+                              void* initial_state_grad, int64_t B, int64_t D, int64_t L, int64_t W, int dtype,
+                              unsigned flags, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token of every row. inputs (B, D) with a row stride, state and state_out (S, D, W-1) dense; state_out may be
+ * state (updated in place) or another pool, of which the named slots alone are written. out (B, D) dense. */
+int fmselective_conv_step(const void* inputs, int64_t batch_stride, const void* state, void* state_out,
+                          const void* weight, const void* bias, const void* slots, void* out, int64_t B, int64_t D,
+                          int64_t W, int64_t S, int dtype, unsigned flags, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif
