@@ -23,6 +23,25 @@ FLAG_SEGMENTS_SHIFT = 20
 SELECTIVE_SOFTPLUS, SELECTIVE_SILU, SELECTIVE_SLOTS_64 = 0x1, 0x2, 0x4
 SELECTIVE_NARROW_WEIGHT, SELECTIVE_NARROW_BIAS, SELECTIVE_NARROW_SKIP = 0x10, 0x20, 0x40
 
+SELECTIVE_MAX_STATES, SELECTIVE_MARK = 256, 128
+
+
+class ScanInputs(ctypes.Structure):
+    """fmselective_scan_inputs"""
+    _fields_ = ([(n, c_void_p) for n in ("tokens", "delta", "gate", "write", "read", "skip", "delta_bias", "A",
+                                         "initial_state", "lengths")]
+                + [(n, c_int64 * 2) for n in ("tokens_strides", "delta_strides", "gate_strides")]
+                + [(n, c_int64 * 3) for n in ("write_strides", "read_strides")]
+                + [(n, c_int64) for n in "BDLNG"] + [("dtype", ctypes.c_int32), ("flags", ctypes.c_uint32)])
+
+
+class ScanGrads(ctypes.Structure):
+    """fmselective_scan_grads"""
+    _fields_ = ([("out_grad", c_void_p), ("out_grad_strides", c_int64 * 2)]
+                + [(n, c_void_p) for n in ("final_state_grad", "marks", "tokens", "delta", "gate", "write", "read", "A",
+                                           "initial_state", "skip", "delta_bias")])
+
+
 _lib = None
 
 
@@ -155,6 +174,14 @@ def load() -> ctypes.CDLL:
     lib.fmselective_conv_step.restype = c_int
     lib.fmselective_conv_step.argtypes = ([c_void_p, c_int64] + [c_void_p] * 6 + [c_int64] * 4
                                           + [c_int, c_uint, c_void_p])
+    lib.fmselective_scan_forward.restype = c_int
+    lib.fmselective_scan_forward.argtypes = [c_void_p] * 5
+    lib.fmselective_scan_workspace_bytes.restype = c_size_t
+    lib.fmselective_scan_workspace_bytes.argtypes = [c_int64] * 5 + [c_int]
+    lib.fmselective_scan_backward.restype = c_int
+    lib.fmselective_scan_backward.argtypes = [c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.fmselective_scan_step.restype = c_int
+    lib.fmselective_scan_step.argtypes = [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]
     got = lib.fmscan_abi_version()
     if got != ABI_VERSION:
         raise RuntimeError(f"libfmscan_hip.so has ABI version {got}, this package needs {ABI_VERSION}; "

@@ -1,0 +1,104 @@
+// The selective scan's forward call and its form for one token. Contract: include/fmselective.h.
+#include "fmselective_scan_host.h"
+
+using namespace fmselective::host;
+using fmselective::Scan;
+
+namespace {
+
+// Lanes a channel: 16, so that a wave works on 4 channels, or all 64, where that leaves too few waves.
+#ifndef FMSELECTIVE_FEW_WAVES
+#define FMSELECTIVE_FEW_WAVES 2048
+#endif
+int lanes_per_channel(const fmselective_scan_inputs& in) {
+    const int64_t waves = in.B * in.G * ((in.D / in.G + 3) / 4);
+    return waves >= FMSELECTIVE_FEW_WAVES || in.L <= 128 ? 16 : 64;
+}
+
+template <typename T, int LPC>
+int launch_forward(const char* who, const fmselective_scan_inputs& in, void* out, float* final_state, float* marks, hipStream_t stream) {
+    constexpr int WAVES = fmselective::kScanWaves;
+    const Scan p = scan_of(in, WAVES * 64 / LPC);
+    const int64_t blocks = in.B * in.G * p.blocks_per_group;
+    if (blocks > INT32_MAX) return fail(FMSCAN_E_SHAPE, "%s: B * D is too large for one launch", who);
+    static std::atomic<uint64_t> armed{0};
+    const size_t lds = fmselective::scan_forward_lds<LPC, WAVES>(p.N);
+    const auto kernel = fmselective::selective_forward_kernel<T, LPC, WAVES>;
+    if (lds > 64 * 1024)
+        if (int rc = raise_lds_limit((const void*)kernel, armed, who)) return rc;
+    kernel<<<(unsigned)blocks, 64 * WAVES, lds, stream>>>(p, (T*)out, final_state, marks);
+    return launched("selective scan (forward)");
+}
+
+}  // namespace
+
+extern "C" {
+
+int fmselective_scan_forward(const fmselective_scan_inputs* in, void* out, float* final_state, float* marks, void* stream) {
+    const char* who = "fmselective_scan_forward";
+    if (int rc = check_scan(who, in, kScanFlags)) return rc;
+    if (!out) return fail(FMSCAN_E_NULL, "%s: out must not be NULL", who);
+    const int64_t states = in->B * in->D * in->N * 4, n_marks = (in->L + fmselective::kMark - 1) / fmselective::kMark;
+    if (int rc = check_outputs(who, {{"out", out, in->B * in->D * in->L * esize_of(in->dtype)}, {"final_state", final_state, states},
+                                     {"marks", marks, states * n_marks}}, input_ranges(*in)))
+        return rc;
+    int rc = 0;
+    with_dtype(in->dtype, [&](auto tt) {
+        using T = typename decltype(tt)::type;
+        rc = lanes_per_channel(*in) == 16 ? launch_forward<T, 16>(who, *in, out, final_state, marks, (hipStream_t)stream)
+                                          : launch_forward<T, 64>(who, *in, out, final_state, marks, (hipStream_t)stream);
+    });
+    return rc;
+}
+
+int fmselective_scan_step(const fmselective_scan_inputs* in, float* state_out, const void* slots, int64_t S, void* out,
+                          void* stream) {
+    const char* who = "fmselective_scan_step";
+    if (!in) return fail(FMSCAN_E_NULL, "%s: the inputs must not be NULL", who);
+    fmselective_scan_inputs one = *in;
+    one.L = 1;
+    if (int rc = check_scan(who, &one, kScanFlags | FMSELECTIVE_SLOTS_64)) return rc;
+    if (int rc = check_pool(who, S, in->B, in->D * in->N, slots)) return rc;
+    if (!in->initial_state || !state_out || !out)
+        return fail(FMSCAN_E_NULL, "%s: initial_state (the pool), state_out and out must not be NULL", who);
+    const int es = esize_of(in->dtype);
+    const int64_t B = in->B, D = in->D, pool = S * D * in->N * 4;
+    auto row = [&](const char* name, const void* p, const int64_t* s) { return Range{name, p, ((B - 1) * s[0] + D) * es}; };
+    auto shared = [&](const char* name, const void* p, const int64_t* s) {
+        return Range{name, p, ((B - 1) * s[0] + (in->G - 1) * s[1] + in->N) * es};
+    };
+    const Range out_r = {"out", out, B * D * es}, new_r = {"state_out", state_out, pool}, old_r = {"the pool", in->initial_state, pool};
+    if (int rc = check_alias(who, {out_r, new_r},
+                             {row("tokens", in->tokens, in->tokens_strides), row("delta", in->delta, in->delta_strides),
+                              row("gate", in->gate, in->gate_strides), shared("write", in->write, in->write_strides),
+                              shared("read", in->read, in->read_strides), {"A", in->A, D * in->N * 4},
+                              {"skip", in->skip, D * (in->flags & FMSELECTIVE_NARROW_SKIP ? es : 4)},
+                              {"delta_bias", in->delta_bias, D * (in->flags & FMSELECTIVE_NARROW_BIAS ? es : 4)},
+                              {"slots", slots, B * (in->flags & FMSELECTIVE_SLOTS_64 ? 8 : 4)}}))
+        return rc;
+    if (int rc = check_alias(who, {out_r}, {old_r})) return rc;
+    if (state_out != in->initial_state)
+        if (int rc = check_alias(who, {new_r}, {old_r})) return rc;
+    fmselective::Step p = {};
+    p.tokens = in->tokens; p.delta = in->delta; p.gate = in->gate; p.write = in->write; p.read = in->read;
+    p.skip = in->skip; p.delta_bias = in->delta_bias; p.slots = slots; p.A = in->A; p.state = in->initial_state;
+    p.state_out = state_out;
+    p.tokens_b = in->tokens_strides[0]; p.delta_b = in->delta_strides[0]; p.gate_b = in->gate_strides[0];
+    p.write_b = in->write_strides[0]; p.write_g = in->write_strides[1];
+    p.read_b = in->read_strides[0]; p.read_g = in->read_strides[1];
+    p.S = S;
+    p.D = (int32_t)D; p.N = (int32_t)in->N; p.per_group = (int32_t)(D / in->G);
+    p.tiles = (uint32_t)((D + 63) / 64);
+    p.flags = in->flags;
+    if ((__int128)B * p.tiles > (__int128)INT32_MAX) return fail(FMSCAN_E_SHAPE, "%s: B * D is too large for one launch", who);
+    const bool vec = in->N % 4 == 0 && aligned16(in->A) && aligned16(in->initial_state) && aligned16(state_out);
+    with_dtype(in->dtype, [&](auto tt) {
+        using T = typename decltype(tt)::type;
+        with_bool(vec, [&](auto vt) {
+            fmselective::selective_step_kernel<T, decltype(vt)::value><<<(unsigned)(B * p.tiles), 256, 0, (hipStream_t)stream>>>(p, (T*)out);
+        });
+    });
+    return launched("selective scan (one token)");
+}
+
+}  // extern "C"

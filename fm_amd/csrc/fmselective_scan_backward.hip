@@ -1,0 +1,112 @@
+// The selective scan's backward call. Contract: include/fmselective.h.
+#include "fmselective_scan_host.h"
+
+using namespace fmselective::host;
+using fmselective::Scan;
+using fmselective::ScanGrads;
+
+namespace {
+
+constexpr int kBackWaves = fmselective::kScanWaves;
+constexpr int kBackChannels = 4 * kBackWaves;
+
+struct BackPlan {
+    int64_t blocks, shared, states, rows;  // blocks; floats of the three kinds of partial sums
+};
+BackPlan plan(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) {
+    const int64_t per_group = D / G, marks = (L + fmselective::kMark - 1) / fmselective::kMark;
+    BackPlan b;
+    b.blocks = B * G * ((per_group + kBackChannels - 1) / kBackChannels);
+    b.shared = b.blocks * N * marks * 256;
+    b.states = B * D * N;
+    b.rows = B * D;
+    return b;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fmselective_scan_workspace_bytes(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int dtype) {
+    if (check_states("fmselective_scan_workspace_bytes", B, D, L, N, G, dtype)) return 0;
+    const BackPlan b = plan(B, D, L, N, G);
+    return (size_t)(b.shared + b.states + 2 * b.rows) * sizeof(float);
+}
+
+int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselective_scan_grads* grads, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+    const char* who = "fmselective_scan_backward";
+    if (int rc = check_scan(who, in, kScanFlags)) return rc;
+    if (!grads) return fail(FMSCAN_E_NULL, "%s: the gradients must not be NULL", who);
+    const fmselective_scan_grads& o = *grads;
+    if (!o.out_grad || !o.marks || !o.tokens || !o.delta || !o.write || !o.read || !o.A || (!o.gate != !in->gate) ||
+        (!o.skip != !in->skip) || (!o.delta_bias != !in->delta_bias))
+        return fail(FMSCAN_E_NULL, "%s: out_grad, marks and every input's gradient must be there, and those of gate, skip and "
+                    "delta_bias where they are", who);
+    for (int i = 0; i < 2; ++i)
+        if (int rc = check_stride(who, "out_grad", o.out_grad_strides[i])) return rc;
+    const BackPlan b = plan(in->B, in->D, in->L, in->N, in->G);
+    const size_t need = fmselective_scan_workspace_bytes(in->B, in->D, in->L, in->N, in->G, in->dtype);
+    if (!workspace || workspace_bytes < need || !aligned16(workspace))
+        return fail(FMSCAN_E_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed (got %zu)", who, need,
+                    workspace ? workspace_bytes : (size_t)0);
+    const int es = esize_of(in->dtype);
+    const int64_t seq = in->B * in->D * in->L * es, shared = in->B * in->G * in->N * in->L * es, states = b.states * 4;
+    const int64_t marks = states * ((in->L + fmselective::kMark - 1) / fmselective::kMark);
+    const Range outs[] = {{"tokens' gradient", o.tokens, seq}, {"delta's gradient", o.delta, seq}, {"gate's gradient", o.gate, seq},
+                          {"write's gradient", o.write, shared}, {"read's gradient", o.read, shared},
+                          {"A's gradient", o.A, in->D * in->N * 4}, {"the initial state's gradient", o.initial_state, states},
+                          {"skip's gradient", o.skip, in->D * (in->flags & FMSELECTIVE_NARROW_SKIP ? es : 4)},
+                          {"delta_bias's gradient", o.delta_bias, in->D * (in->flags & FMSELECTIVE_NARROW_BIAS ? es : 4)},
+                          {"workspace", workspace, (int64_t)need}};
+    const Range more[] = {{"out_grad", o.out_grad, extent(in->B, in->D, in->L, o.out_grad_strides[0], o.out_grad_strides[1], es)},
+                          {"final_state_grad", o.final_state_grad, states}, {"marks", o.marks, marks}};
+    const InputRanges ins = input_ranges(*in);
+    for (const Range& r : outs) {
+        if (int rc = check_outputs(who, {r}, ins)) return rc;
+        if (int rc = check_alias(who, {r}, {more[0], more[1], more[2]})) return rc;
+        for (const Range& q : outs)
+            if (&q != &r && overlap(q, r)) return fail(FMSCAN_E_ALIAS, "%s: %s overlaps %s", who, r.name, q.name);
+    }
+    const Scan p = scan_of(*in, kBackChannels);
+    const int64_t lines = in->B * in->G * in->N, waves = lines * p.marks;
+    if (b.blocks > INT32_MAX || waves > (int64_t)INT32_MAX * 4)
+        return fail(FMSCAN_E_SHAPE, "%s: B * D or B * G * N * L is too large for one launch", who);
+    float* part = (float*)workspace;
+    ScanGrads g = {};
+    g.out_grad = o.out_grad;
+    g.out_b = o.out_grad_strides[0];
+    g.out_d = o.out_grad_strides[1];
+    g.final_grad = o.final_state_grad;
+    g.marks = o.marks;
+    g.tokens = o.tokens;
+    g.delta = o.delta;
+    g.gate = o.gate;
+    g.initial = o.initial_state;
+    g.shared_part = part;
+    g.A_part = part + b.shared;
+    g.skip_part = o.skip ? part + b.shared + b.states : nullptr;
+    g.bias_part = o.delta_bias ? part + b.shared + b.states + b.rows : nullptr;
+    int rc = 0;
+    with_dtype(in->dtype, [&](auto tt) {
+        using T = typename decltype(tt)::type;
+        static std::atomic<uint64_t> armed{0};
+        const size_t lds = fmselective::scan_backward_lds<kBackWaves>(p.N);
+        const auto kernel = fmselective::selective_backward_kernel<T, kBackWaves>;
+        if (lds > 64 * 1024 && (rc = raise_lds_limit((const void*)kernel, armed, who))) return;
+        kernel<<<(unsigned)b.blocks, 64 * kBackWaves, lds, (hipStream_t)stream>>>(p, g);
+        if ((rc = launched("selective scan (backward)"))) return;
+        fmselective::selective_shared_grads_kernel<T><<<(unsigned)((waves + 3) / 4), 256, 0, (hipStream_t)stream>>>(
+            part, (T*)o.write, (T*)o.read, in->lengths, in->L, waves, p.N, p.G, p.marks, p.blocks_per_group);
+        rc = launched("selective scan (gradients of write and read)");
+    });
+    if (rc) return rc;
+    launch_column_sums(in->dtype,
+                       {{g.A_part, o.A, in->B, in->D * in->N, 0, 0},
+                        {g.skip_part, o.skip, in->B, in->D, (in->flags & FMSELECTIVE_NARROW_SKIP) != 0, 0},
+                        {g.bias_part, o.delta_bias, in->B, in->D, (in->flags & FMSELECTIVE_NARROW_BIAS) != 0, 0}},
+                       (hipStream_t)stream);
+    return launched("selective scan (sums of the parameters' gradients)");
+}
+
+}  // extern "C"

@@ -11,13 +11,15 @@ implementation behind them. The reference has no counterpart of these operators.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .fm_scan import _dtype_code, _on_device, _on_gpu, _ptr, _raw, _require
 
-__all__ = ["fm_conv", "fm_conv_step", "FM_Conv"]
+__all__ = ["fm_conv", "fm_conv_step", "FM_Conv", "fm_selective_scan", "fm_selective_step", "FM_Selective"]
 
 
 def _stream(dev):
@@ -219,4 +221,193 @@ def fm_conv_step(inputs, state, weight, bias=None, slots=None, silu=True, state_
             _lib.check(_raw.fmselective_conv_step(
                 inputs.data_ptr(), inputs.stride(0), state.data_ptr(), new.data_ptr(), weight.data_ptr(), _ptr(bias),
                 _ptr(slots), out.data_ptr(), B, D, W, state.shape[0], code, flags, _stream(dev)))
+    return out
+
+
+def _scan_inputs(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus):
+    """The checked arguments of a call on sequences, as the library takes them."""
+    _require(tokens.dim() == 3 and A.dim() == 2 and write.dim() == 4, "tokens must be (B, D, L), A (D, N), write (B, G, N, L)")
+    B, D, L = tokens.shape
+    N, G = A.shape[1], write.shape[1]
+    dev = tokens.device
+    _sequence("tokens", tokens, tokens.shape, tokens)
+    code = _dtype_code(tokens)
+    _sequence("delta", delta, tokens.shape, tokens)
+    _require(1 <= N <= _lib.SELECTIVE_MAX_STATES, f"A must have 1 to {_lib.SELECTIVE_MAX_STATES} states, got {N}")
+    _dense("A", A, (D, N), torch.float32, dev)
+    _require(G >= 1 and D % G == 0, f"the groups of write must divide the {D} channels, got {G}")
+    _sequence("write", write, (B, G, N, L), tokens)
+    _sequence("read", read, (B, G, N, L), tokens)
+    flags = _lib.SELECTIVE_SOFTPLUS if softplus else 0
+    if skip is not None:
+        flags |= _parameter("skip", skip, (D,), tokens, _lib.SELECTIVE_NARROW_SKIP)
+    if delta_bias is not None:
+        flags |= _parameter("delta_bias", delta_bias, (D,), tokens, _lib.SELECTIVE_NARROW_BIAS)
+    if gate is not None:
+        _sequence("gate", gate, tokens.shape, tokens)
+    if initial_state is not None:
+        _dense("initial_state", initial_state, (B, D, N), torch.float32, dev)
+    _lengths(lengths, B, dev)
+    return _lib.ScanInputs(
+        tokens.data_ptr(), delta.data_ptr(), _ptr(gate), write.data_ptr(), read.data_ptr(), _ptr(skip), _ptr(delta_bias),
+        A.data_ptr(), _ptr(initial_state), _ptr(lengths), tokens.stride()[:2], delta.stride()[:2],
+        (0, 0) if gate is None else gate.stride()[:2], write.stride()[:3], read.stride()[:3], B, D, L, N, G, code, flags)
+
+
+def _scan_forward(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus, return_state, save):
+    """(out, final state or None, the states that backward starts from or None)"""
+    p = _scan_inputs(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus)
+    dev = tokens.device
+    out = torch.empty((p.B, p.D, p.L), dtype=tokens.dtype, device=dev)
+    if not out.numel():
+        return out, _carried(initial_state, (p.B, p.D, p.N), tokens, torch.float32) if return_state else None, None
+    final = torch.empty((p.B, p.D, p.N), dtype=torch.float32, device=dev) if return_state else None
+    marks = None
+    if save:
+        marks = torch.empty((p.B, p.D, -(-p.L // _lib.SELECTIVE_MARK), p.N), dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        _lib.check(_raw.fmselective_scan_forward(ctypes.addressof(p), out.data_ptr(), _ptr(final), _ptr(marks), _stream(dev)))
+    return out, final, marks
+
+
+def _scan_backward(inputs, softplus, marks, out_grad, final_grad, want_state):
+    """Gradients in the order of the inputs, None for absent ones."""
+    tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths = inputs
+    p = _scan_inputs(*inputs, softplus)
+    dev, dtype = tokens.device, tokens.dtype
+    shape = (p.B, p.D, p.L)
+    if out_grad is None:
+        out_grad = torch.zeros(shape, dtype=dtype, device=dev)
+    elif out_grad.stride(-1) != 1:
+        out_grad = out_grad.contiguous()
+    _sequence("the output's gradient", out_grad, shape, tokens)
+    if final_grad is not None:
+        final_grad = final_grad.contiguous()
+        _dense("the final state's gradient", final_grad, (p.B, p.D, p.N), torch.float32, dev)
+    if not tokens.numel():
+        d_state = None
+        if want_state:
+            d_state = torch.zeros((p.B, p.D, p.N), dtype=torch.float32, device=dev) if final_grad is None else final_grad
+        zeros = [None if t is None else torch.zeros_like(t) for t in (tokens, delta, A, write, read, skip, gate, delta_bias)]
+        return (*zeros, d_state)
+    new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
+    grads = [new(t) for t in (tokens, delta, A, write, read, skip, gate, delta_bias)]
+    d_tokens, d_delta, d_A, d_write, d_read, d_skip, d_gate, d_bias = grads
+    d_state = torch.empty((p.B, p.D, p.N), dtype=torch.float32, device=dev) if want_state else None
+    need = _raw.fmselective_scan_workspace_bytes(p.B, p.D, p.L, p.N, p.G, p.dtype)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    o = _lib.ScanGrads(out_grad.data_ptr(), out_grad.stride()[:2], _ptr(final_grad), marks.data_ptr(), d_tokens.data_ptr(),
+                       d_delta.data_ptr(), _ptr(d_gate), d_write.data_ptr(), d_read.data_ptr(), d_A.data_ptr(),
+                       _ptr(d_state), _ptr(d_skip), _ptr(d_bias))
+    with _on_device(dev):
+        _lib.check(_raw.fmselective_scan_backward(ctypes.addressof(p), ctypes.addressof(o), workspace.data_ptr(), need,
+                                                  _stream(dev)))
+    return (*grads, d_state)
+
+
+class FM_Selective(torch.autograd.Function):
+    """out, final_state = FM_Selective.apply(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state,
+    lengths, softplus, return_state): fm_selective_scan with write and read (B, G, N, L); final_state is None
+    unless asked for."""
+
+    @staticmethod
+    def forward(ctx, tokens, delta, A, write, read, skip=None, gate=None, delta_bias=None, initial_state=None, lengths=None,
+                softplus=True, return_state=False):
+        inputs = (tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths)
+        save = any(ctx.needs_input_grad)
+        out, final, marks = _scan_forward(*inputs, softplus, return_state, save)
+        if save:
+            ctx.save_for_backward(*inputs, marks)
+            ctx.softplus = bool(softplus)
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, out_grad, final_grad):
+        *inputs, marks = ctx.saved_tensors
+        if out_grad is None and final_grad is None:
+            return (None,) * 12
+        grads = _scan_backward(inputs, ctx.softplus, marks, out_grad, final_grad, ctx.needs_input_grad[8])
+        return (*grads, None, None, None)
+
+
+def fm_selective_scan(tokens, delta, A, write, read, skip=None, gate=None, delta_bias=None, initial_state=None, lengths=None,
+                      softplus=True, return_state=False):
+    """Selective state space scan: N states a channel, whose decay depends on channel, state and step.
+
+        dt = softplus(delta + delta_bias)
+        h[b, d, n] <- exp(dt * A[d, n]) * h[b, d, n] + dt * tokens[b, d, t] * write[b, g, n, t]
+        out[b, d, t] = (sum_n read[b, g, n, t] * h[b, d, n] + skip[d] * tokens[b, d, t]) * silu(gate[b, d, t])
+
+    Arguments:
+        tokens, delta (B, D, L) and gate (B, D, L) or None: one dtype, time stride 1, any batch and channel stride.
+        A (D, N): float32, negative in a model whose states decay; N up to 256.
+        write, read (B, G, N, L), or (B, N, L) for one group: of the tokens' dtype, time stride 1; channel d is in
+            group g = d // (D / G).
+        skip, delta_bias (D,): float32 or the tokens' dtype; absent is zero.
+        initial_state (B, D, N): float32; zeros if omitted.
+        lengths (B,) int32: the steps that count of each row of a padded batch (clamped to [0, L]); nothing is read
+            beyond them, the output is zero there, and the final state is that after the last step that counts.
+        softplus: apply it to delta + delta_bias, else the sum is dt itself.
+        return_state: also return the state after the last step that counts, float32 (B, D, N).
+
+    Returns (B, D, L) of the tokens' dtype, or that and the final state. Differentiable once, in everything but lengths.
+    """
+    if write.dim() == 3 and read.dim() == 3:
+        write, read = write.unsqueeze(1), read.unsqueeze(1)
+    out, final = FM_Selective.apply(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus,
+                                    return_state)
+    return (out, final) if return_state else out
+
+
+def fm_selective_step(tokens, state, delta, A, write, read, skip=None, gate=None, delta_bias=None, slots=None, softplus=True,
+                      state_out=None):
+    """fm_selective_scan for one token of every row; moves the state on by it. Not differentiable.
+
+    Arguments:
+        tokens, delta, gate (B, D): channel stride 1. write, read (B, G, N) or (B, N): state stride 1.
+        state (S, D, N): float32 pool of states, updated in place.
+        slots (B,) int32 or int64: which state a row has; S = B and row b has state b if omitted. A row whose slot
+            lies outside [0, S) is skipped: its output is zero and no state is touched. Where a slot is named more
+            than once the first row has it and the others are skipped.
+        state_out (S, D, N): where the named states are written instead (`state` then stays as it is: the way back
+            when a token is not accepted).
+
+    Returns (B, D) of the tokens' dtype.
+    """
+    if write.dim() == 2 and read.dim() == 2:
+        write, read = write.unsqueeze(1), read.unsqueeze(1)
+    _require(tokens.dim() == 2 and A.dim() == 2 and write.dim() == 3, "tokens must be (B, D), A (D, N), write (B, G, N)")
+    B, D = tokens.shape
+    N, G = A.shape[1], write.shape[1]
+    dev = tokens.device
+    _sequence("tokens", tokens, tokens.shape, tokens)
+    code = _dtype_code(tokens)
+    _sequence("delta", delta, tokens.shape, tokens)
+    _require(1 <= N <= _lib.SELECTIVE_MAX_STATES, f"A must have 1 to {_lib.SELECTIVE_MAX_STATES} states, got {N}")
+    _dense("A", A, (D, N), torch.float32, dev)
+    _require(G >= 1 and D % G == 0, f"the groups of write must divide the {D} channels, got {G}")
+    _sequence("write", write, (B, G, N), tokens)
+    _sequence("read", read, (B, G, N), tokens)
+    flags = (_lib.SELECTIVE_SOFTPLUS if softplus else 0) | _slots(slots, B, dev)
+    if skip is not None:
+        flags |= _parameter("skip", skip, (D,), tokens, _lib.SELECTIVE_NARROW_SKIP)
+    if delta_bias is not None:
+        flags |= _parameter("delta_bias", delta_bias, (D,), tokens, _lib.SELECTIVE_NARROW_BIAS)
+    if gate is not None:
+        _sequence("gate", gate, tokens.shape, tokens)
+    new = _pool(state, state_out, slots, B, (D, N), torch.float32, dev)
+    if slots is not None and state.shape[0] == 0:
+        return torch.zeros((B, D), dtype=tokens.dtype, device=dev)
+    out = torch.empty((B, D), dtype=tokens.dtype, device=dev)
+    if out.numel():
+        p = _lib.ScanInputs(
+            tokens.data_ptr(), delta.data_ptr(), _ptr(gate), write.data_ptr(), read.data_ptr(), _ptr(skip),
+            _ptr(delta_bias), A.data_ptr(), state.data_ptr(), None, (tokens.stride(0), 0), (delta.stride(0), 0),
+            (0 if gate is None else gate.stride(0), 0), (write.stride(0), write.stride(1), 0),
+            (read.stride(0), read.stride(1), 0), B, D, 1, N, G, code, flags)
+        with _on_device(dev):
+            _lib.check(_raw.fmselective_scan_step(ctypes.addressof(p), new.data_ptr(), _ptr(slots), state.shape[0],
+                                                  out.data_ptr(), _stream(dev)))
     return out

@@ -69,6 +69,54 @@ int fmselective_conv_step(const void* inputs, int64_t batch_stride, const void* 
                           const void* weight, const void* bias, const void* slots, void* out, int64_t B, int64_t D,
                           int64_t W, int64_t S, int dtype, unsigned flags, void* stream);
 
+/* ---- selective scan ------------------------------------------------------------------------------------
+ *   dt = softplus(delta + delta_bias),  h[b,d,n] <- exp(dt A[d,n]) h[b,d,n] + dt tokens[b,d,t] write[b,g,n,t]
+ *   out[b,d,t] = (sum_n read[b,g,n,t] h[b,d,n] + skip[d] tokens[b,d,t]) * silu(gate[b,d,t])
+ * with channel d in group g = d / (D / G). tokens, delta, gate (B, D, L) and write, read (B, G, N, L) have one
+ * element type and any strides but the time's, which is 1; A (D, N), states and their gradients are float32.
+ * gate, skip, delta_bias, initial_state and lengths may be NULL. 1 <= N <= FMSELECTIVE_MAX_STATES, G divides D. */
+#define FMSELECTIVE_MAX_STATES 256
+#define FMSELECTIVE_MARK 128 /* steps between the states that forward saves for backward */
+
+typedef struct fmselective_scan_inputs {
+    const void *tokens, *delta, *gate, *write, *read, *skip, *delta_bias;
+    const float *A, *initial_state;
+    const int32_t* lengths;
+    int64_t tokens_strides[2], delta_strides[2], gate_strides[2]; /* batch, channel */
+    int64_t write_strides[3], read_strides[3];                    /* batch, group, state */
+    int64_t B, D, L, N, G;
+    int32_t dtype;
+    uint32_t flags;
+} fmselective_scan_inputs;
+
+/* out (B, D, L); final_state (B, D, N) or NULL; marks (B, D, ceil(L / FMSELECTIVE_MARK), N) float32 or NULL: the
+ * states before every FMSELECTIVE_MARK steps, which the backward call needs (those at or beyond a row's length
+ * are not written). */
+int fmselective_scan_forward(const fmselective_scan_inputs* in, void* out, float* final_state, float* marks, void* stream);
+
+typedef struct fmselective_scan_grads {
+    const void* out_grad;           /* (B, D, L), strided */
+    int64_t out_grad_strides[2];
+    const float* final_state_grad;  /* (B, D, N) or NULL */
+    const float* marks;             /* as forward wrote them */
+    void *tokens, *delta, *gate;    /* (B, D, L) dense; gate NULL where the inputs' is */
+    void *write, *read;             /* (B, G, N, L) dense */
+    float *A, *initial_state;       /* (D, N); (B, D, N) or NULL */
+    void *skip, *delta_bias;        /* (D), of the parameters' types, NULL where the inputs' are */
+} fmselective_scan_grads;
+
+/* Bytes of workspace that the backward call needs (partial sums over channels and batch); 0 where sizes are not valid. */
+size_t fmselective_scan_workspace_bytes(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int dtype);
+int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselective_scan_grads* grads, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* One token of every row. tokens, delta, gate (B, D) with a row stride (tokens_strides[0], ...), write and read
+ * (B, G, N) with a batch and a group stride (the first two), L and lengths unused, initial_state the pool
+ * (S, D, N) dense. state_out may be the pool (updated in place) or another, of which the named slots alone are
+ * written. out (B, D) dense. */
+int fmselective_scan_step(const fmselective_scan_inputs* in, float* state_out, const void* slots, int64_t S, void* out,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

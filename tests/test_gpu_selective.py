@@ -173,3 +173,78 @@ def test_conv_steps_are_the_sequence(m):
     for t in range(12):
         assert torch.equal(m.fm_conv_step(x[..., t].contiguous(), state, w, bias), whole[..., t])
     assert torch.equal(state, last)
+
+
+# ---- selective scan ---------------------------------------------------------------------------------
+# The reference's magnitudes follow every term through the recurrence, a rounding a step and the decay's own error
+# included. On top of those a result passes through the composition of 8 steps, of 16 or 64 lanes and of the tiles
+# (products of decays in place of one step after the other: at most 6 levels of two roundings each and the total's
+# exponent, three roundings of |dt A| summed), the sum over N, and about ten operations of softplus (twice) and
+# gate: c = 40 + N. A gradient multiplies two such quantities and runs both ways: c = 80 + 2 N; sums over time, channels
+# and batch add a rounding for every term that one thread adds: 8 steps a tile, L / 128 tiles, 16 blocks.
+
+SCAN_SHAPES = [  # B, D, L, N, G
+    (1, 1, 1, 1, 1), (2, 3, 2, 2, 1), (1, 4, 7, 3, 2), (2, 6, 9, 16, 3), (3, 17, 40, 5, 1), (1, 8, 127, 16, 2),
+    (1, 33, 128, 8, 1), (2, 20, 129, 17, 1), (1, 5, 300, 33, 1), (2, 4, 513, 4, 4), (1, 2, 1100, 16, 1), (70, 2, 3, 4, 1)]
+
+
+def scan_case(shape, dtype, variant, seed=0):
+    B, D, L, N, G = shape
+    g = gen(B * 100 + D * 10 + L + N + variant + seed)
+    a = {"tokens": rand(g, B, D, L, dtype=dtype), "delta": rand(g, B, D, L, dtype=dtype, scale=0.5),
+         "A": -torch.exp(rand(g, D, N)) * (1 + torch.arange(N, device=DEV)) / 4,
+         "write": rand(g, B, G, N, L, dtype=dtype), "read": rand(g, B, G, N, L, dtype=dtype)}
+    a["skip"] = rand(g, D, dtype=dtype if variant == 2 else F32) if variant else None
+    a["gate"] = rand(g, B, D, L, dtype=dtype) if variant != 1 else None
+    a["delta_bias"] = rand(g, D, dtype=dtype if variant == 1 else F32) - 3 if variant != 2 else None
+    a["initial_state"] = rand(g, B, D, N) if variant >= 2 else None
+    a["lengths"] = None
+    dy, dfinal = rand(g, B, D, L, dtype=dtype), rand(g, B, D, N)
+    if variant == 3:
+        n = torch.randint(0, L + 1, (B,), generator=g, dtype=torch.int32)
+        n[0] = (L, 0, L + 7, -2)[L % 4]
+        a["lengths"] = n.to(DEV)
+        for k in ("tokens", "delta", "gate", "write", "read"):
+            spoil(a[k], n)
+        spoil(dy, n)
+    if variant in (1, 3):
+        for k in ("tokens", "delta", "gate"):
+            if a[k] is not None:
+                a[k] = strided(a[k])
+        for k in ("write", "read"):
+            a[k] = strided(a[k].flatten(1, 2), pad_batch=0).unflatten(1, (G, N))
+        dy = strided(dy)
+    return a, dy, dfinal, variant != 2 or None
+
+
+REF = {"tokens": "u", "initial_state": "state", "delta_bias": "bias"}
+GRADS = {"tokens": "du", "delta": "ddelta", "A": "dA", "write": "dwrite", "read": "dread", "skip": "dskip", "gate": "dgate",
+         "delta_bias": "dbias", "initial_state": "dstate"}
+
+
+def scan_reference(a, softplus, dy=None, dfinal=None):
+    return R.scan(**{REF.get(k, k): v for k, v in a.items()}, softplus=softplus, dy=dy, dfinal=dfinal)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", SCAN_SHAPES, ids=str)
+def test_selective_scan(m, shape, dtype):
+    B, D, L, N, G = shape
+    for variant in range(4):
+        a, dy, dfinal, softplus = scan_case(shape, dtype, variant)
+        softplus = bool(softplus)
+        if not softplus:
+            a["delta"] = a["delta"].abs() * 0.2
+        what = f"{shape} {dtype} variant {variant}"
+        ref = scan_reference(a, softplus, dy, dfinal)
+        y, final = m.fm_selective_scan(**a, softplus=softplus, return_state=True)
+        R.close(y, *ref["y"], 40 + N, what + " y")
+        R.close(final, *ref["final"], 40 + N, what + " final")
+        leaves = {k: v.requires_grad_() for k, v in a.items() if v is not None and k != "lengths"}
+        y2, final2 = m.fm_selective_scan(**a, softplus=softplus, return_state=True)
+        assert torch.equal(y, y2) and torch.equal(final, final2)
+        grads = torch.autograd.grad([y2, final2], list(leaves.values()), [dy, dfinal])
+        c = 80 + 2 * N + 16 + 8 + L / 128 + B
+        for k, t in zip(leaves, grads):
+            assert t.dtype == a[k].dtype
+            R.close(t, *ref[GRADS[k]], c, f"{what} {GRADS[k]}")
