@@ -23,7 +23,7 @@ FLAG_SEGMENTS_SHIFT = 20
 SELECTIVE_SOFTPLUS, SELECTIVE_SILU, SELECTIVE_SLOTS_64 = 0x1, 0x2, 0x4
 SELECTIVE_NARROW_WEIGHT, SELECTIVE_NARROW_BIAS, SELECTIVE_NARROW_SKIP = 0x10, 0x20, 0x40
 
-SELECTIVE_MAX_STATES, SELECTIVE_MARK = 256, 128
+SELECTIVE_MAX_STATES, SELECTIVE_MARK, SELECTIVE_MAX_NORM = 256, 128, 16384
 
 
 class ScanInputs(ctypes.Structure):
@@ -182,6 +182,13 @@ def load() -> ctypes.CDLL:
     lib.fmselective_scan_backward.argtypes = [c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
     lib.fmselective_scan_step.restype = c_int
     lib.fmselective_scan_step.argtypes = [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]
+    lib.fmselective_norm_forward.restype = c_int
+    lib.fmselective_norm_forward.argtypes = [c_void_p] * 7 + [c_int64] * 2 + [c_int, c_uint, c_float, c_void_p]
+    lib.fmselective_norm_workspace_bytes.restype = c_size_t
+    lib.fmselective_norm_workspace_bytes.argtypes = [c_int64] * 2 + [c_int]
+    lib.fmselective_norm_backward.restype = c_int
+    lib.fmselective_norm_backward.argtypes = ([c_void_p] * 7 + [c_int64] * 2
+                                              + [c_int, c_uint, c_void_p, c_size_t, c_void_p])
     got = lib.fmscan_abi_version()
     if got != ABI_VERSION:
         raise RuntimeError(f"libfmscan_hip.so has ABI version {got}, this package needs {ABI_VERSION}; "

@@ -26,10 +26,10 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 UNITS = ["fmscan_core.hip", "fmscan_forward.hip", "fmscan_backward.hip", "fmscan_reduced.hip",
          "fmscan_readout.hip", "fmscan_normed.hip", "fmselective_conv.hip", "fmselective_scan.hip",
-         "fmselective_scan_backward.hip"]
+         "fmselective_scan_backward.hip", "fmselective_norm.hip"]
 HEADERS = ["fmscan_host.h", "fmscan_device.h", "fmscan_kernels.h", "fmscan_reduced.h", "fmscan_readout.h",
            "fmscan_normed.h", "fmscan_packed.h", "fmselective_host.h", "fmselective_device.h", "fmselective_conv.h",
-           "fmselective_scan.h", "fmselective_scan_host.h"]
+           "fmselective_scan.h", "fmselective_scan_host.h", "fmselective_norm.h"]
 DEPS = [CSRC / n for n in UNITS + HEADERS] + [PKG.parent / "include" / n for n in ("fmscan.h", "fmselective.h")]
 LIB = PKG / "lib" / "libfmscan_hip.so"
 HIPCC_FLAGS = [

@@ -3,6 +3,7 @@
 // Contract of the calls: include/fmselective.h.
 #pragma once
 
+#include "../../include/fmselective.h"
 #include "fmscan_device.h"
 
 namespace fmselective {
@@ -92,7 +93,7 @@ constexpr int kSumSections = 3;
 struct ColumnSums {
     ColumnSum part[kSumSections];
 };
-constexpr int kSumWaves = 8;
+constexpr int kSumWaves = 16;
 
 template <typename T>
 __global__ __launch_bounds__(64 * kSumWaves) void column_sums_kernel(ColumnSums s) {
@@ -105,7 +106,7 @@ __global__ __launch_bounds__(64 * kSumWaves) void column_sums_kernel(ColumnSums 
     const int64_t c = (int64_t)(blockIdx.x - p.first_block) * 64 + lane;
     float sum = 0.0f;
     if (c < p.cols) {
-#pragma unroll 4
+#pragma unroll 8
         for (int64_t i = wave; i < p.n; i += kSumWaves) sum += p.src[i * p.cols + c];
     }
     __shared__ float shared[kSumWaves][64];

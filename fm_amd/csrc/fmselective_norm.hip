@@ -1,0 +1,121 @@
+// The norm's entry points: forward (also in 8 bits) and backward. Contract: include/fmselective.h.
+#include "fmselective_host.h"
+#include "fmselective_norm.h"
+
+using namespace fmselective::host;
+
+namespace {
+
+constexpr unsigned kNormFlags = FMSELECTIVE_NARROW_WEIGHT;
+
+int check_rows(const char* who, int64_t rows, int64_t D, int dtype) {
+    if (rows < 1 || D < 1 || rows > INT32_MAX)
+        return fail(FMSCAN_E_SHAPE, "%s: rows and D must be >= 1 and rows fit 31 bits (got %lld, %lld)", who, (long long)rows,
+                    (long long)D);
+    if (dtype != FMSCAN_DTYPE_F32 && dtype != FMSCAN_DTYPE_F16 && dtype != FMSCAN_DTYPE_BF16)
+        return fail(FMSCAN_E_DTYPE, "%s: dtype %d is not float32 (0), float16 (1) or bfloat16 (2)", who, dtype);
+    if (D > FMSELECTIVE_MAX_NORM)
+        return fail(FMSCAN_E_SHAPE, "%s: D must be at most %d (got %lld)", who, FMSELECTIVE_MAX_NORM, (long long)D);
+    return 0;
+}
+
+// Threads a row and chunks a thread: a wave up to 2 chunks a lane, then a block of 256 up to 4, then one of 1024.
+template <typename F>
+void with_row_shape(int64_t D, int dtype, F&& f) {
+    const int64_t chunks = (D + (dtype == FMSCAN_DTYPE_F32 ? 4 : 8) - 1) / (dtype == FMSCAN_DTYPE_F32 ? 4 : 8);
+    if (chunks <= 64) f(IntTag<64>{}, IntTag<1>{});
+    else if (chunks <= 128) f(IntTag<64>{}, IntTag<2>{});
+    else if (chunks <= 256) f(IntTag<256>{}, IntTag<1>{});
+    else if (chunks <= 512) f(IntTag<256>{}, IntTag<2>{});
+    else if (chunks <= 1024) f(IntTag<256>{}, IntTag<4>{});
+    else if (chunks <= 2048) f(IntTag<1024>{}, IntTag<2>{});
+    else f(IntTag<1024>{}, IntTag<4>{});  // FMSELECTIVE_MAX_NORM float32 values are 4096 chunks
+}
+
+// Rows that work side by side in the backward call, each slot with its part of the weight's gradient: enough for
+// the memory's latency, few enough that the parts are small beside the streams.
+constexpr int64_t kNormSlots = 512;
+int64_t backward_slots(int64_t rows) {
+    int64_t n = (rows + 7) / 8;
+    return n > kNormSlots ? kNormSlots : n;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fmselective_norm_forward(const void* inputs, const void* residual, const void* weight, void* residual_out, void* out,
+                             float* scales, float* inv_rms, int64_t rows, int64_t D, int dtype, unsigned flags, float eps,
+                             void* stream) {
+    const char* who = "fmselective_norm_forward";
+    if (int rc = check_rows(who, rows, D, dtype)) return rc;
+    if (int rc = check_flags(who, flags, kNormFlags)) return rc;
+    if (!(eps >= 0.0f)) return fail(FMSCAN_E_SHAPE, "%s: eps must be >= 0", who);
+    if (!inputs || !weight || !out || (residual && !residual_out))
+        return fail(FMSCAN_E_NULL, "%s: inputs, weight, out, and residual_out with a residual, must not be NULL", who);
+    const int es = esize_of(dtype);
+    if (int rc = check_alias(who,
+                             {{"out", out, rows * D * (scales ? 1 : es)}, {"residual_out", residual ? residual_out : nullptr, rows * D * es},
+                              {"scales", scales, rows * 4}, {"inv_rms", inv_rms, rows * 4}},
+                             {{"inputs", inputs, rows * D * es}, {"residual", residual, rows * D * es},
+                              {"weight", weight, D * (flags & FMSELECTIVE_NARROW_WEIGHT ? es : 4)}}))
+        return rc;
+    with_dtype(dtype, [&](auto tt) {
+        using T = typename decltype(tt)::type;
+        with_row_shape(D, dtype, [&](auto pt, auto ct) {
+            constexpr int TPR = decltype(pt)::value, CH = decltype(ct)::value, RPB = TPR == 64 ? 4 : 1;
+            with_bool(scales != nullptr, [&](auto qt) {
+                fmselective::norm_forward_kernel<T, TPR, CH, decltype(qt)::value>
+                    <<<(unsigned)((rows + RPB - 1) / RPB), TPR == 64 ? 256 : TPR, 0, (hipStream_t)stream>>>(
+                        (const T*)inputs, (const T*)residual, weight, (T*)residual_out, out, scales, inv_rms, rows, (int32_t)D,
+                        eps, flags);
+            });
+        });
+    });
+    return launched("norm (forward)");
+}
+
+size_t fmselective_norm_workspace_bytes(int64_t rows, int64_t D, int dtype) {
+    if (check_rows("fmselective_norm_workspace_bytes", rows, D, dtype)) return 0;
+    // (short rows go four to a block: whole blocks of four slots)
+    return (size_t)((backward_slots(rows) + 3) / 4 * 4) * D * sizeof(float);
+}
+
+int fmselective_norm_backward(const void* out_grad, const void* residual_grad, const void* stream_in, const void* weight,
+                              const float* inv_rms, void* grad, void* weight_grad, int64_t rows, int64_t D, int dtype,
+                              unsigned flags, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "fmselective_norm_backward";
+    if (int rc = check_rows(who, rows, D, dtype)) return rc;
+    if (int rc = check_flags(who, flags, kNormFlags)) return rc;
+    if (!out_grad || !stream_in || !weight || !inv_rms || !grad || !weight_grad)
+        return fail(FMSCAN_E_NULL, "%s: out_grad, the stream, weight, inv_rms and the gradients must not be NULL", who);
+    const size_t need = fmselective_norm_workspace_bytes(rows, D, dtype);
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 3u))
+        return fail(FMSCAN_E_WORKSPACE, "%s: a 4-byte aligned workspace of %zu bytes is needed (got %zu)", who, need,
+                    workspace ? workspace_bytes : (size_t)0);
+    const int es = esize_of(dtype), ws = flags & FMSELECTIVE_NARROW_WEIGHT ? es : 4;
+    if (int rc = check_alias(who,
+                             {{"grad", grad, rows * D * es}, {"weight_grad", weight_grad, D * ws},
+                              {"workspace", workspace, (int64_t)need}},
+                             {{"out_grad", out_grad, rows * D * es}, {"residual_grad", residual_grad, rows * D * es},
+                              {"the stream", stream_in, rows * D * es}, {"weight", weight, D * ws}, {"inv_rms", inv_rms, rows * 4}}))
+        return rc;
+    int64_t slots = backward_slots(rows);
+    with_dtype(dtype, [&](auto tt) {
+        using T = typename decltype(tt)::type;
+        with_row_shape(D, dtype, [&](auto pt, auto ct) {
+            constexpr int TPR = decltype(pt)::value, CH = decltype(ct)::value, RPB = TPR == 64 ? 4 : 1;
+            const int64_t blocks = (slots + RPB - 1) / RPB;
+            slots = blocks * RPB;
+            fmselective::norm_backward_kernel<T, TPR, CH><<<(unsigned)blocks, TPR == 64 ? 256 : TPR, 0, (hipStream_t)stream>>>(
+                (const T*)out_grad, (const T*)residual_grad, (const T*)stream_in, weight, inv_rms, (T*)grad, (float*)workspace,
+                rows, (int32_t)D, flags);
+        });
+    });
+    if (int rc = launched("norm (backward)")) return rc;
+    launch_column_sums(dtype, {{(const float*)workspace, weight_grad, slots, D, (flags & FMSELECTIVE_NARROW_WEIGHT) != 0, 0}},
+                       (hipStream_t)stream);
+    return launched("norm (the weight's gradient)");
+}
+
+}  // extern "C"

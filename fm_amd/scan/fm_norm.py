@@ -1,0 +1,122 @@
+"""Root-mean-square norm over the last axis with the residual's addition, on MI355X: the entry of a block around
+`fm_memory` or `fm_selective_scan`.
+
+    fm_norm             differentiable, output in the inputs' dtype
+    fm_norm_quantized   output in 8 bits (e4m3) with one scale a row, for a product in 8 bits
+
+float32, float16 and bfloat16; statistics and gradient sums in float32. The kernels are in libfmscan_hip.so
+(include/fmselective.h); there is no CPU implementation behind them. The reference normalises inside its layer alone
+(fm/scan/fm_scan.py:124-127).
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from .fm_scan import _dtype_code, _on_device, _on_gpu, _ptr, _raw, _require
+
+__all__ = ["fm_norm", "fm_norm_quantized", "FM_Norm"]
+
+
+def _check(inputs, weight, residual, eps):
+    """(rows, D, dtype code, flags)"""
+    _require(inputs.dim() >= 1 and weight.dim() == 1, "inputs must be (..., D) and weight (D,)")
+    dev, dtype, D = inputs.device, inputs.dtype, inputs.shape[-1]
+    _on_gpu("inputs", inputs, dev)
+    code = _dtype_code(inputs)
+    _require(inputs.is_contiguous(), "inputs must be contiguous")
+    _require(D <= _lib.SELECTIVE_MAX_NORM, f"the last axis must have at most {_lib.SELECTIVE_MAX_NORM} elements, got {D}")
+    _on_gpu("weight", weight, dev)
+    _require(weight.dtype == torch.float32 or weight.dtype == dtype,
+             f"weight has dtype {weight.dtype}, expected torch.float32 or {dtype}")
+    _require(weight.shape == (D,) and weight.is_contiguous(), f"weight must be a dense {(D,)}, got {tuple(weight.shape)}")
+    _require(eps >= 0, f"eps must be >= 0, got {eps}")
+    if residual is not None:
+        _on_gpu("residual", residual, dev)
+        _require(residual.dtype == dtype, f"residual has dtype {residual.dtype}, expected {dtype}")
+        _require(residual.shape == inputs.shape, f"residual must be {tuple(inputs.shape)}, got {tuple(residual.shape)}")
+        _require(residual.is_contiguous(), "residual must be contiguous")
+    return inputs.numel() // D if D else 0, D, code, 0 if weight.dtype == torch.float32 else _lib.SELECTIVE_NARROW_WEIGHT
+
+
+def _forward(inputs, weight, residual, eps, save=False, quantized=False):
+    """(out, residual_out or None, inv_rms or None, scales or None)"""
+    rows, D, code, flags = _check(inputs, weight, residual, eps)
+    dev = inputs.device
+    out = torch.empty(inputs.shape, dtype=torch.float8_e4m3fn if quantized else inputs.dtype, device=dev)
+    stream_out = None if residual is None else torch.empty_like(inputs)
+    inv_rms = torch.empty(rows, dtype=torch.float32, device=dev) if save else None
+    scales = torch.empty(inputs.shape[:-1], dtype=torch.float32, device=dev) if quantized else None
+    if rows:
+        with _on_device(dev):
+            _lib.check(_raw.fmselective_norm_forward(
+                inputs.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(stream_out), out.data_ptr(), _ptr(scales),
+                _ptr(inv_rms), rows, D, code, flags, float(eps), torch.cuda.current_stream(dev).cuda_stream))
+    elif quantized:
+        scales.zero_()
+    return out, stream_out, inv_rms, scales
+
+
+class FM_Norm(torch.autograd.Function):
+    """out, residual_out = FM_Norm.apply(inputs, weight, residual, eps); residual_out is None without a residual."""
+
+    @staticmethod
+    def forward(ctx, inputs, weight, residual=None, eps=1e-6):
+        save = any(ctx.needs_input_grad)
+        out, stream_out, inv_rms, _ = _forward(inputs, weight, residual, eps, save=save)
+        if save:
+            ctx.save_for_backward(inputs if residual is None else stream_out, weight, inv_rms)
+        ctx.set_materialize_grads(False)
+        return out, stream_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, out_grad, residual_grad):
+        stream_in, weight, inv_rms = ctx.saved_tensors
+        if out_grad is None and residual_grad is None:
+            return None, None, None, None
+        if out_grad is None:  # nothing goes through the norm
+            return residual_grad, torch.zeros_like(weight), residual_grad, None
+        rows, D, code, flags = _check(stream_in, weight, None, 0.0)
+        dev = stream_in.device
+        grad, d_weight = torch.empty_like(stream_in), torch.empty_like(weight)
+        if not rows:
+            return grad, d_weight.zero_(), grad, None
+        out_grad = out_grad.contiguous()
+        residual_grad = None if residual_grad is None else residual_grad.contiguous()
+        need = _raw.fmselective_norm_workspace_bytes(rows, D, code)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        with _on_device(dev):
+            _lib.check(_raw.fmselective_norm_backward(
+                out_grad.data_ptr(), _ptr(residual_grad), stream_in.data_ptr(), weight.data_ptr(), inv_rms.data_ptr(),
+                grad.data_ptr(), d_weight.data_ptr(), rows, D, code, flags, workspace.data_ptr(), need,
+                torch.cuda.current_stream(dev).cuda_stream))
+        return grad, d_weight, grad if ctx.needs_input_grad[2] else None, None
+
+
+def fm_norm(inputs, weight, residual=None, eps=1e-6):
+    """Root-mean-square norm of inputs + residual over the last axis, and the sum itself.
+
+        r = inputs + residual (in the inputs' dtype),  out = r / sqrt(mean(r ** 2) + eps) * weight
+
+    Arguments:
+        inputs, residual (..., D): contiguous, one dtype; residual may be omitted (r is inputs then). D up to 16384.
+        weight (D,): float32 or the inputs' dtype.
+
+    Returns (out (..., D), r (..., D)): r is the residual of the next block. What the norm sees is r as it is
+    stored, rounded. Differentiable once, in inputs, weight and residual.
+    """
+    out, stream_out = FM_Norm.apply(inputs, weight, residual, eps)
+    return out, (inputs if residual is None else stream_out)
+
+
+def fm_norm_quantized(inputs, weight, residual=None, eps=1e-6):
+    """fm_norm with its output in 8 bits, one scale a row. Not differentiable.
+
+    Returns (values (..., D) torch.float8_e4m3fn, scales (...) float32, r (..., D)): out is values * scales, scales are
+    max |out| / 448 of each row, values are rounded to nearest even. A row of zeros, or of values below 2^-100, has scale
+    0; a row with a NaN among its outputs has a NaN scale.
+    """
+    out, stream_out, _, scales = _forward(inputs, weight, residual, eps, quantized=True)
+    return out, scales, (inputs if residual is None else stream_out)

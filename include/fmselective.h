@@ -117,6 +117,27 @@ int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselecti
 int fmselective_scan_step(const fmselective_scan_inputs* in, float* state_out, const void* slots, int64_t S, void* out,
                           void* stream);
 
+/* ---- root-mean-square norm with the residual's addition ------------------------------------------------
+ *   r = inputs + residual (rounded to the element type, as it is stored), inv = 1 / sqrt(mean r^2 + eps)
+ *   out = r inv weight
+ * over `rows` dense rows of D elements, 1 <= D <= FMSELECTIVE_MAX_NORM. residual may be NULL (r is inputs, nothing
+ * is stored). inv_rms (rows) float32 may be NULL; the backward call needs it. With scales (rows) float32 the output
+ * is 8-bit e4m3 instead, one byte an element: scales = max |out| / 448 of the row, values out / scale rounded to
+ * nearest even (a row of zeros, or of values below 2^-100, has scale 0 and zeros; one with a NaN among its outputs
+ * has a NaN scale). */
+#define FMSELECTIVE_MAX_NORM 16384
+int fmselective_norm_forward(const void* inputs, const void* residual, const void* weight, void* residual_out, void* out,
+                             float* scales, float* inv_rms, int64_t rows, int64_t D, int dtype, unsigned flags, float eps,
+                             void* stream);
+
+size_t fmselective_norm_workspace_bytes(int64_t rows, int64_t D, int dtype);
+
+/* stream_in: r as forward stored it (the inputs without a residual). residual_grad: the gradient that arrives at r
+ * from elsewhere, or NULL. grad: that of inputs and of residual, which is the same. */
+int fmselective_norm_backward(const void* out_grad, const void* residual_grad, const void* stream_in, const void* weight,
+                              const float* inv_rms, void* grad, void* weight_grad, int64_t rows, int64_t D, int dtype,
+                              unsigned flags, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

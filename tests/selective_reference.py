@@ -164,3 +164,20 @@ def scan(u, delta, A, write, read, skip=None, gate=None, bias=None, state=None, 
         dslope = sig * (1 + z * (1 - sig))
         out["dgate"] = (mask(dy * y * dslope), mask(dy.abs() * ymag * (dslope.abs() + z.abs() + 1)))
     return out
+
+
+def norm(r, w, eps, dy=None, dr=None):
+    """The norm of the stored stream r (..., D) and its gradients: {name: (value, magnitude)}."""
+    r, w, dy, dr = (f64(v) for v in (r, w, dy, dr))
+    inv = 1 / (r.pow(2).mean(-1, keepdim=True) + eps).sqrt()
+    y = r * inv * w
+    out = {"y": (y, y.abs())}
+    if dy is None and dr is None:
+        return out
+    x, gw = r * inv, (torch.zeros_like(r) if dy is None else dy) * w
+    dr = torch.zeros_like(r) if dr is None else dr
+    out["dr"] = (dr + inv * (gw - x * (gw * x).mean(-1, keepdim=True)),
+                 dr.abs() + inv * (gw.abs() + x.abs() * (gw * x).abs().mean(-1, keepdim=True)))
+    rows = lambda v: v.reshape(-1, v.shape[-1]).sum(0)  # noqa: E731
+    out["dweight"] = (rows(dy * x), rows((dy * x).abs()))
+    return out

@@ -132,3 +132,124 @@ def test_conv_checks_its_arguments(monkeypatch):
         (dict(state_out=torch.rand(4, D, 3)), "state_out must be"),
         (dict(inputs=torch.rand(D, B).t()), "time stride"),
     ])
+
+
+def scan_inputs(_lib, **change):
+    a = dict(tokens=P, delta=2 * P, gate=None, write=3 * P, read=4 * P, skip=None, delta_bias=None, A=5 * P, initial_state=None,
+             lengths=None, tokens_strides=(24, 8), delta_strides=(24, 8), gate_strides=(24, 8), write_strides=(32, 32, 8),
+             read_strides=(32, 32, 8), B=2, D=3, L=8, N=4, G=1, dtype=2, flags=0)
+    return _lib.ScanInputs(**{**a, **change})
+
+
+def test_scan_rejects(lib):
+    import ctypes
+
+    from fm_amd import _lib
+
+    def fwd(out=7 * P, final=None, marks=None, **change):
+        p = scan_inputs(_lib, **change)
+        return lib.fmselective_scan_forward(ctypes.addressof(p), out, final, marks, None)
+
+    assert lib.fmselective_scan_forward(None, P, None, None, None) == code("NULL")
+    assert fwd(out=None) == code("NULL") and fwd(tokens=None) == code("NULL") and fwd(read=None) == code("NULL")
+    assert fwd(N=0) == code("SHAPE") and fwd(N=257) == code("SHAPE") and fwd(G=2) == code("SHAPE") and fwd(L=0) == code("SHAPE")
+    assert fwd(write_strides=(32, 32, -8)) == code("SHAPE") and fwd(B=1 << 30, D=4) == code("SHAPE")
+    assert fwd(dtype=5) == code("DTYPE") and fwd(flags=0x4) == code("FLAGS") and fwd(flags=0x2) == code("FLAGS")
+    assert fwd(out=P + 32) == code("ALIAS") and fwd(final=5 * P) == code("ALIAS") and fwd(marks=7 * P) == code("ALIAS")
+    assert fwd(initial_state=6 * P, final=6 * P) == code("ALIAS")
+    need = lib.fmselective_scan_workspace_bytes
+    assert need(2, 3, 8, 4, 1, 2) > 0 and need(2, 3, 8, 4, 2, 2) == 0 and need(2, 3, 0, 4, 1, 2) == 0
+
+    def bwd(ws=20 * P, ws_bytes=1 << 30, inputs={}, **change):
+        g = dict(out_grad=7 * P, out_grad_strides=(24, 8), final_state_grad=None, marks=8 * P, tokens=9 * P, delta=10 * P,
+                 gate=None, write=11 * P, read=12 * P, A=13 * P, initial_state=None, skip=None, delta_bias=None)
+        p, o = scan_inputs(_lib, **inputs), _lib.ScanGrads(**{**g, **change})
+        return lib.fmselective_scan_backward(ctypes.addressof(p), ctypes.addressof(o), ws, ws_bytes, None)
+
+    assert bwd(marks=None) == code("NULL") and bwd(write=None) == code("NULL")
+    assert bwd(gate=14 * P) == code("NULL") and bwd(inputs=dict(skip=15 * P)) == code("NULL")
+    assert bwd(ws=None) == code("WORKSPACE") and bwd(ws_bytes=64) == code("WORKSPACE") and bwd(ws=20 * P + 4) == code("WORKSPACE")
+    assert bwd(tokens=7 * P) == code("ALIAS") and bwd(delta=9 * P) == code("ALIAS") and bwd(ws=13 * P) == code("ALIAS")
+
+    def step(state=6 * P, new=6 * P, slots=None, S=2, out=7 * P, **change):
+        p = scan_inputs(_lib, initial_state=state, **change)
+        return lib.fmselective_scan_step(ctypes.addressof(p), new, slots, S, out, None)
+
+    assert step(state=None) == code("NULL") and step(out=None) == code("NULL")
+    assert step(S=3) == code("SHAPE") and step(S=0, slots=16 * P) == code("SHAPE") and step(new=6 * P + 16) == code("ALIAS")
+    assert step(out=6 * P) == code("ALIAS") and step(N=300) == code("SHAPE") and step(flags=0x8) == code("FLAGS")
+
+
+def test_norm_rejects(lib):
+    def fwd(x=P, r=None, w=2 * P, ro=None, out=3 * P, s=None, inv=None, rows=4, D=8, dtype=2, flags=0, eps=1e-6):
+        return lib.fmselective_norm_forward(x, r, w, ro, out, s, inv, rows, D, dtype, flags, eps, None)
+
+    assert fwd(x=None) == code("NULL") and fwd(r=4 * P) == code("NULL") and fwd(rows=0) == code("SHAPE") and fwd(D=16385) == code("SHAPE")
+    assert fwd(eps=-1.0) == code("SHAPE") and fwd(eps=float("nan")) == code("SHAPE") and fwd(dtype=9) == code("DTYPE")
+    assert fwd(flags=1) == code("FLAGS") and fwd(out=P) == code("ALIAS") and fwd(r=4 * P, ro=4 * P) == code("ALIAS")
+    assert fwd(s=3 * P + 8) == code("ALIAS") and fwd(inv=2 * P) == code("ALIAS")
+
+    def bwd(dy=P, dr=None, x=2 * P, w=3 * P, inv=4 * P, g=5 * P, dw=6 * P, ws=7 * P, n=1 << 20):
+        return lib.fmselective_norm_backward(dy, dr, x, w, inv, g, dw, 4, 8, 2, 0, ws, n, None)
+
+    assert bwd(inv=None) == code("NULL") and bwd(ws=None) == code("WORKSPACE") and bwd(n=4) == code("WORKSPACE")
+    assert bwd(g=P) == code("ALIAS") and bwd(dr=5 * P) == code("ALIAS") and bwd(ws=6 * P) == code("ALIAS")
+
+
+def test_scan_checks_its_arguments(monkeypatch):
+    import fm_amd.scan.fm_selective as m
+
+    on_cpu(monkeypatch, [m])
+    B, D, L, N = 2, 6, 8, 4
+    r = torch.rand
+    good = dict(tokens=r(B, D, L), delta=r(B, D, L), A=r(D, N), write=r(B, 2, N, L), read=r(B, 2, N, L), skip=r(D), gate=r(B, D, L),
+                delta_bias=r(D), initial_state=r(B, D, N), lengths=torch.tensor([1, 8], dtype=torch.int32))
+    refuses(m.fm_selective_scan, good, [
+        (dict(tokens=r(B, L, D).transpose(1, 2)), "tokens must have a time stride"),
+        (dict(delta=r(B, D, L + 1)), "delta must be"),
+        (dict(delta=r(B, D, L).half()), "delta has dtype"),
+        (dict(A=r(D, N).half()), "A has dtype"),
+        (dict(A=r(D, 257), write=r(B, 2, 257, L), read=r(B, 2, 257, L)), "states"),
+        (dict(write=r(B, 4, N, L), read=r(B, 4, N, L)), "groups"),
+        (dict(read=r(B, 1, N, L)), "read must be"),
+        (dict(write=r(B, N, L)), "write"),
+        (dict(write=r(B, 2, L, N).transpose(2, 3)), "write must have a time stride"),
+        (dict(skip=r(D + 1)), "skip must be"),
+        (dict(gate=r(B, D, L).to("meta")), "gate is on meta"),
+        (dict(delta_bias=r(D).double()), "delta_bias has dtype"),
+        (dict(initial_state=r(B, D, N).half()), "initial_state has dtype"),
+        (dict(initial_state=r(B, N, D).transpose(1, 2)), "initial_state must be contiguous"),
+        (dict(lengths=torch.tensor([1, 8])), "lengths has dtype"),
+    ])
+    good = dict(tokens=r(B, D), state=r(5, D, N), delta=r(B, D), A=r(D, N), write=r(B, N), read=r(B, N), gate=r(B, D),
+                slots=torch.tensor([0, 4]))
+    refuses(m.fm_selective_step, good, [
+        (dict(slots=None), "without slots"),
+        (dict(slots=torch.tensor([0, 4], dtype=torch.int16)), "slots has dtype"),
+        (dict(state=r(5, D, N).half()), "state has dtype"),
+        (dict(state=r(5, N, D).transpose(1, 2)), "state must be contiguous"),
+        (dict(state_out=r(5, D, N + 1)), "state_out must be"),
+        (dict(write=r(B, N + 1)), "write must be"),
+        (dict(gate=r(D, B).t()), "gate must have"),
+        (dict(tokens=r(B, D, 1)), "must be"),
+    ])
+
+
+def test_norm_checks_its_arguments(monkeypatch):
+    import fm_amd.scan.fm_norm as m
+
+    on_cpu(monkeypatch, [m])
+    r = torch.rand
+    good = dict(inputs=r(2, 3, 8), weight=r(8), residual=r(2, 3, 8))
+    for call in (m.fm_norm, m.fm_norm_quantized):
+        refuses(call, good, [
+            (dict(inputs=r(2, 8, 3).transpose(1, 2)), "inputs must be contiguous"),
+            (dict(inputs=r(2, 3, 8).double()), "dtype"),
+            (dict(weight=r(9)), "weight must be"),
+            (dict(weight=r(8).half()), "weight has dtype"),
+            (dict(residual=r(2, 3, 9)), "residual must be"),
+            (dict(residual=r(2, 3, 8).half()), "residual has dtype"),
+            (dict(residual=r(2, 8, 3).transpose(1, 2)), "residual must be contiguous"),
+            (dict(eps=-1e-6), "eps"),
+            (dict(inputs=r(1, 16385), weight=r(16385), residual=None), "16384"),
+        ])
