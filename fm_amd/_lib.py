@@ -7,6 +7,7 @@ on a GPU are rejected.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_uint, c_void_p
 
 from . import build as _build
@@ -26,20 +27,13 @@ SELECTIVE_NARROW_WEIGHT, SELECTIVE_NARROW_BIAS, SELECTIVE_NARROW_SKIP = 0x10, 0x
 SELECTIVE_MAX_STATES, SELECTIVE_MARK, SELECTIVE_MAX_NORM = 256, 128, 16384
 
 
-class ScanInputs(ctypes.Structure):
-    """fmselective_scan_inputs"""
-    _fields_ = ([(n, c_void_p) for n in ("tokens", "delta", "gate", "write", "read", "skip", "delta_bias", "A",
-                                         "initial_state", "lengths")]
-                + [(n, c_int64 * 2) for n in ("tokens_strides", "delta_strides", "gate_strides")]
-                + [(n, c_int64 * 3) for n in ("write_strides", "read_strides")]
-                + [(n, c_int64) for n in "BDLNG"] + [("dtype", ctypes.c_int32), ("flags", ctypes.c_uint32)])
-
-
-class ScanGrads(ctypes.Structure):
-    """fmselective_scan_grads"""
-    _fields_ = ([("out_grad", c_void_p), ("out_grad_strides", c_int64 * 2)]
-                + [(n, c_void_p) for n in ("final_state_grad", "marks", "tokens", "delta", "gate", "write", "read", "A",
-                                           "initial_state", "skip", "delta_bias")])
+# fmselective_scan_inputs: tokens, delta, gate, write, read, skip, delta_bias, A, initial_state, lengths; the strides of
+# tokens, delta, gate (batch, channel) and of write, read (batch, group, state); B, D, L, N, G; dtype, flags.
+# Packed into bytes: half the time of a ctypes structure, which a call for one token would notice.
+SCAN_INPUTS = struct.Struct("10Q12q5qiI")
+# fmselective_scan_grads: out_grad, its strides; final_state_grad, marks, tokens, delta, gate, write, read, A,
+# initial_state, skip, delta_bias
+SCAN_GRADS = struct.Struct("Q2q11Q")
 
 
 _lib = None
@@ -175,9 +169,9 @@ def load() -> ctypes.CDLL:
     lib.fmselective_conv_step.argtypes = ([c_void_p, c_int64] + [c_void_p] * 6 + [c_int64] * 4
                                           + [c_int, c_uint, c_void_p])
     lib.fmselective_scan_forward.restype = c_int
-    lib.fmselective_scan_forward.argtypes = [c_void_p] * 5
+    lib.fmselective_scan_forward.argtypes = [c_void_p] * 5 + [c_size_t, c_void_p]
     lib.fmselective_scan_workspace_bytes.restype = c_size_t
-    lib.fmselective_scan_workspace_bytes.argtypes = [c_int64] * 5 + [c_int]
+    lib.fmselective_scan_workspace_bytes.argtypes = [c_int64] * 5 + [c_int, c_int]
     lib.fmselective_scan_backward.restype = c_int
     lib.fmselective_scan_backward.argtypes = [c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
     lib.fmselective_scan_step.restype = c_int

@@ -39,47 +39,62 @@ struct Scan {
     int64_t tokens_b, tokens_d, delta_b, delta_d, gate_b, gate_d, write_b, write_g, write_n, read_b, read_g, read_n;
     int64_t L;
     int32_t D, N, G, per_group, blocks_per_group, marks;  // marks: ceil(L / kMark)
+    int32_t segments, seg_tiles;  // a row's tiles are dealt to `segments` blocks, seg_tiles each
+    int64_t rows;                 // B D
+    float2* pairs;                // (segment, B D, N): what a segment does to a state (or a gradient) that enters it
     uint32_t flags;
 };
 
-// Two rows' worth of (decay, value) pairs, composed over the lanes of a row of 16 (and, with LPC = 64, over the
-// rows): on exit a lane holds the composition of its own and all earlier lanes' pairs. Two pairs at a time: the
-// instructions of one fill the two wait states that the other needs between a write and a DPP read.
-#define FMSELECTIVE_LEVEL(CTRL)                                          \
-    "v_fmac_f32_dpp %1, %1, %0 " CTRL "\n\t"                             \
-    "v_fmac_f32_dpp %3, %3, %2 " CTRL "\n\t"                             \
-    "v_mul_f32_dpp %0, %0, %0 " CTRL "\n\t"                              \
-    "v_mul_f32_dpp %2, %2, %2 " CTRL "\n\t"
+// (decay, value) pairs composed over the lanes of a channel: on exit a lane holds the composition of its own and
+// all earlier lanes' pairs. A register written by a VALU instruction may be read through DPP two wait states later
+// at the earliest: the pair's other instruction is one, the s_nop the other.
+#define FMSELECTIVE_LEVEL(A, B, CTRL)                     \
+    "v_fmac_f32_dpp " B ", " B ", " A " " CTRL "\n\t"     \
+    "v_mul_f32_dpp " A ", " A ", " A " " CTRL "\n\t"
 template <int LPC>
-__device__ __forceinline__ void scan_up(float& a0, float& b0, float& a1, float& b1) {
+__device__ __forceinline__ void scan_up(float& a, float& b) {
     if constexpr (LPC == 16)
         asm("s_nop 1\n\t"
-            FMSELECTIVE_LEVEL("row_shr:1 row_mask:0xf bank_mask:0xf")
-            FMSELECTIVE_LEVEL("row_shr:2 row_mask:0xf bank_mask:0xf")
-            FMSELECTIVE_LEVEL("row_shr:4 row_mask:0xf bank_mask:0xf")
-            FMSELECTIVE_LEVEL("row_shr:8 row_mask:0xf bank_mask:0xf")
+            FMSELECTIVE_LEVEL("%0", "%1", "row_shr:1 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
+            FMSELECTIVE_LEVEL("%0", "%1", "row_shr:2 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
+            FMSELECTIVE_LEVEL("%0", "%1", "row_shr:4 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
+            FMSELECTIVE_LEVEL("%0", "%1", "row_shr:8 row_mask:0xf bank_mask:0xf")
             "s_nop 1"
-            : "+v"(a0), "+v"(b0), "+v"(a1), "+v"(b1));
+            : "+v"(a), "+v"(b));
     else
         asm("s_nop 1\n\t"
-            FMSELECTIVE_LEVEL("row_shr:1 row_mask:0xf bank_mask:0xf")
-            FMSELECTIVE_LEVEL("row_shr:2 row_mask:0xf bank_mask:0xf")
-            FMSELECTIVE_LEVEL("row_shr:4 row_mask:0xf bank_mask:0xf")
-            FMSELECTIVE_LEVEL("row_shr:8 row_mask:0xf bank_mask:0xf")
-            FMSELECTIVE_LEVEL("row_bcast:15 row_mask:0xa bank_mask:0xf")
-            FMSELECTIVE_LEVEL("row_bcast:31 row_mask:0xc bank_mask:0xf")
+            FMSELECTIVE_LEVEL("%0", "%1", "row_shr:1 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
+            FMSELECTIVE_LEVEL("%0", "%1", "row_shr:2 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
+            FMSELECTIVE_LEVEL("%0", "%1", "row_shr:4 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
+            FMSELECTIVE_LEVEL("%0", "%1", "row_shr:8 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
+            FMSELECTIVE_LEVEL("%0", "%1", "row_bcast:15 row_mask:0xa bank_mask:0xf") "s_nop 0\n\t"
+            FMSELECTIVE_LEVEL("%0", "%1", "row_bcast:31 row_mask:0xc bank_mask:0xf")
             "s_nop 1"
-            : "+v"(a0), "+v"(b0), "+v"(a1), "+v"(b1));
+            : "+v"(a), "+v"(b));
 }
-// The same towards lower lanes, inside rows of 16
-__device__ __forceinline__ void scan_down(float& a0, float& b0, float& a1, float& b1) {
+__device__ __forceinline__ void scan_down(float& a, float& b) {
     asm("s_nop 1\n\t"
-        FMSELECTIVE_LEVEL("row_shl:1 row_mask:0xf bank_mask:0xf")
-        FMSELECTIVE_LEVEL("row_shl:2 row_mask:0xf bank_mask:0xf")
-        FMSELECTIVE_LEVEL("row_shl:4 row_mask:0xf bank_mask:0xf")
-        FMSELECTIVE_LEVEL("row_shl:8 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LEVEL("%0", "%1", "row_shl:1 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
+        FMSELECTIVE_LEVEL("%0", "%1", "row_shl:2 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
+        FMSELECTIVE_LEVEL("%0", "%1", "row_shl:4 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
+        FMSELECTIVE_LEVEL("%0", "%1", "row_shl:8 row_mask:0xf bank_mask:0xf")
         "s_nop 1"
-        : "+v"(a0), "+v"(b0), "+v"(a1), "+v"(b1));
+        : "+v"(a), "+v"(b));
+}
+// One pair towards higher lanes and one towards lower lanes, inside rows of 16: the two scans fill each other's
+// wait states.
+__device__ __forceinline__ void scan_both(float& up_a, float& up_b, float& down_a, float& down_b) {
+    asm("s_nop 1\n\t"
+        FMSELECTIVE_LEVEL("%0", "%1", "row_shr:1 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LEVEL("%2", "%3", "row_shl:1 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LEVEL("%0", "%1", "row_shr:2 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LEVEL("%2", "%3", "row_shl:2 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LEVEL("%0", "%1", "row_shr:4 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LEVEL("%2", "%3", "row_shl:4 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LEVEL("%0", "%1", "row_shr:8 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LEVEL("%2", "%3", "row_shl:8 row_mask:0xf bank_mask:0xf")
+        "s_nop 1"
+        : "+v"(up_a), "+v"(up_b), "+v"(down_a), "+v"(down_b));
 }
 #undef FMSELECTIVE_LEVEL
 
@@ -125,48 +140,109 @@ __device__ __forceinline__ void widen_raw(const Raw<T>& r, float (&f)[kSteps]) {
 
 // The shared tile of write and read: for each of NC states, LPC chunks of 8 steps, the chunks' first and second
 // halves in planes of their own so that the lanes of a row read whole lines of banks.
-template <int LPC, int WAVES>
+template <int LPC, int NC>
 struct SharedTile {
-    static constexpr int kStates = 64 * WAVES / LPC;  // states in LDS at a time: one chunk of each operand a thread
-    float v[2][kStates][2][LPC][4];                   // write / read, state, half, chunk, step
-    __device__ __forceinline__ void put(int which, const float (&f)[kSteps]) {
-        const int n = threadIdx.x / LPC, c = threadIdx.x % LPC;
-        *reinterpret_cast<float4*>(v[which][n][0][c]) = make_float4(f[0], f[1], f[2], f[3]);
-        *reinterpret_cast<float4*>(v[which][n][1][c]) = make_float4(f[4], f[5], f[6], f[7]);
+    alignas(16) float v[2][NC][2][LPC][4];  // write / read, state, half, chunk, step
+};
+// Steps of a lane out of the tile: `at` points to the lane's four floats of a state of `write`
+template <int LPC>
+__device__ __forceinline__ void steps_at(const float* at, float (&f)[kSteps]) {
+    const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 4 * LPC);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+
+// A thread's part of filling the tile: one or two chunks of 16-bit or 32-bit steps, loaded a tile ahead
+template <typename T, int LPC, int NC, int WAVES>
+struct TileLoader {
+    static constexpr int kChunks = NC * LPC, kEach = 2 * kChunks / (64 * WAVES);
+    static_assert(kEach >= 1 && 2 * kChunks % (64 * WAVES) == 0, "whole chunks a thread");
+    Raw<T> raw[kEach];
+    __device__ __forceinline__ void load(const T* write, int64_t write_n, const T* read, int64_t read_n, int n0, int N,
+                                         int64_t tile_t0, int64_t len) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const int i = threadIdx.x + j * 64 * WAVES, which = i / kChunks, n = n0 + (i / LPC) % NC, c = i % LPC;
+            const T* rows = which ? read + n * read_n : write + n * write_n;
+            raw[j] = load_raw<T>(rows, tile_t0 + c * kSteps, n < N ? len : 0);
+        }
     }
-    __device__ __forceinline__ void get(int which, int n, int c, float (&f)[kSteps]) const {
-        const float4 a = *reinterpret_cast<const float4*>(v[which][n][0][c]);
-        const float4 b = *reinterpret_cast<const float4*>(v[which][n][1][c]);
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    __device__ __forceinline__ void put(SharedTile<LPC, NC>& t) const {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const int i = threadIdx.x + j * 64 * WAVES, which = i / kChunks, n = (i / LPC) % NC, c = i % LPC;
+            float f[kSteps];
+            widen_raw(raw[j], f);
+            *reinterpret_cast<float4*>(t.v[which][n][0][c]) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4*>(t.v[which][n][1][c]) = make_float4(f[4], f[5], f[6], f[7]);
+        }
     }
 };
 
-// states of a channel in LDS: an even number, the one beyond N with no decay and no value
-__host__ __device__ __forceinline__ int padded_states(int N) { return (N + 1) & ~1; }
-// and the stride between channels, in entries: odd, so that channels do not share banks
-__host__ __device__ __forceinline__ int state_stride(int N) { return padded_states(N) | 1; }
+// entries between the states of two channels in LDS: odd, so that channels do not share banks
+__host__ __device__ __forceinline__ int state_stride(int N) { return N | 1; }
 
+// Forward keeps two tiles of kStates states in LDS (one being filled), backward one
 template <int LPC, int WAVES>
-constexpr size_t scan_tiles_bytes() { return 2 * sizeof(SharedTile<LPC, WAVES>); }
+constexpr int tile_states() { return LPC == 16 ? 16 : WAVES; }
 template <int LPC, int WAVES>
-size_t scan_forward_lds(int N) { return scan_tiles_bytes<LPC, WAVES>() + (size_t)WAVES * (64 / LPC) * state_stride(N) * sizeof(float2); }
+size_t scan_forward_lds(int N) {
+    return 2 * sizeof(SharedTile<LPC, tile_states<LPC, WAVES>()>) + (size_t)WAVES * (64 / LPC) * state_stride(N) * sizeof(float2);
+}
 
-template <typename T, int LPC, int WAVES>
+// Steps that count among the 8 from t0
+__device__ __forceinline__ int steps_left(int64_t len, int64_t t0) {
+    const int64_t n = len - t0;
+    return n < 0 ? 0 : (n > kSteps ? kSteps : (int)n);
+}
+
+// The block's part of the problem
+struct Place {
+    uint32_t b, g, block;
+    int32_t seg;
+    int64_t line;  // of the block without its segment
+};
+__device__ __forceinline__ Place place_of(const Scan& p) {
+    Place w;
+    const uint32_t line = p.segments == 1 ? blockIdx.x : blockIdx.x / (uint32_t)p.segments;
+    w.seg = (int32_t)(blockIdx.x - line * p.segments);
+    const uint32_t bg = line / (uint32_t)p.blocks_per_group;
+    w.block = line - bg * p.blocks_per_group;
+    w.b = bg / (uint32_t)p.G;
+    w.g = bg - w.b * p.G;
+    w.line = line;
+    return w;
+}
+
+// dt of a lane's steps from the raw delta
+__device__ __forceinline__ void steps_of(float (&dt)[kSteps], float bias, uint32_t flags, bool ragged, int left) {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) dt[k] += bias;
+    if (flags & FMSELECTIVE_SOFTPLUS) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) dt[k] = softplus(dt[k]);
+    }
+    if (ragged) {  // a step of length zero leaves the state as it is
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) dt[k] = k < left ? dt[k] : 0.0f;
+    }
+}
+
+// Forward over the tiles of a segment. Where rows are too few to fill the GPU they are cut into segments: a first
+// launch (ENDS) finds what each segment but the last does to a state, without the outputs; the second composes
+// the segments before its own, as many multiply-adds a state, and then runs as for a whole row.
+template <typename T, int LPC, int WAVES, bool ENDS>
 __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T* __restrict__ out, float* __restrict__ final_state,
                                                                        float* __restrict__ marks) {
-    using Tile = SharedTile<LPC, WAVES>;
-    constexpr int NC = Tile::kStates, kTile = LPC * kSteps, CW = 64 / LPC;
-    extern __shared__ char lds[];
+    constexpr int NC = tile_states<LPC, WAVES>(), kTile = LPC * kSteps, CW = 64 / LPC;
+    using Tile = SharedTile<LPC, NC>;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     Tile* tiles = reinterpret_cast<Tile*>(lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & (LPC - 1), ch = lane / LPC;
-    const int stride = state_stride(p.N);
-    float2* held = reinterpret_cast<float2*>(lds + scan_tiles_bytes<LPC, WAVES>()) + wave * CW * stride;  // (A log2 e, state)
 
-    const uint32_t bg = blockIdx.x / (uint32_t)p.blocks_per_group, block = blockIdx.x - bg * p.blocks_per_group;
-    const uint32_t b = bg / (uint32_t)p.G, g = bg - b * p.G;
-    const int32_t first = (int32_t)(block * WAVES + wave) * CW;  // the wave's first channel in the group
-    const int32_t local = first + ch;
+    const Place w = place_of(p);
+    const uint32_t b = w.b, g = w.g;
+    const int32_t local = (int32_t)(w.block * WAVES + wave) * CW + ch;  // the lane's channel in the group
     const bool valid = local < p.per_group;
     const int32_t d = (int32_t)g * p.per_group + (valid ? local : p.per_group - 1);
     const int64_t row = (int64_t)b * p.D + d;
@@ -179,153 +255,141 @@ __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T
     const float skip = p.skip ? param<T>(p.skip, d, p.flags & FMSELECTIVE_NARROW_SKIP) : 0.0f;
     const float bias = p.delta_bias ? param<T>(p.delta_bias, d, p.flags & FMSELECTIVE_NARROW_BIAS) : 0.0f;
 
-    // decay rates and entering states of the wave's channels
-    const int padded = padded_states(p.N);
-    auto each_state = [&](auto&& f) {  // f(entry in `held`, its channel's row or -1, n) over the wave's lanes
-        for (int i = lane; i < CW * padded; i += 64) {
-            const int k = i / padded, n = i - k * padded;
-            const bool real = n < p.N && first + k < p.per_group;
-            f(held[k * stride + n], real ? (int64_t)b * p.D + (int64_t)g * p.per_group + first + k : (int64_t)-1, n);
+    // the lane's channel's decay rates (A log2 e) and the states that enter the tile
+    float2* held = reinterpret_cast<float2*>(lds + 2 * sizeof(Tile)) + (wave * CW + ch) * state_stride(p.N);
+    for (int n = c; n < p.N; n += LPC) {
+        float h = !ENDS && valid && p.initial ? p.initial[row * p.N + n] : 0.0f;
+        if (!ENDS && valid) {
+#pragma unroll 4
+            for (int32_t j = 0; j < w.seg; ++j) {
+                const float2 q = p.pairs[(j * p.rows + row) * p.N + n];
+                h = __builtin_fmaf(q.x, h, q.y);
+            }
         }
-    };
-    each_state([&](float2& e, int64_t r, int n) {
-        e.x = r < 0 ? 0.0f : p.A[(r - (int64_t)b * p.D) * p.N + n] * kLog2E;
-        e.y = r < 0 || !p.initial ? 0.0f : p.initial[r * p.N + n];
-    });
+        held[n] = make_float2(p.A[(int64_t)d * p.N + n] * kLog2E, h);
+    }
 
     const int chunks = (p.N + NC - 1) / NC;
-    const int32_t n_tiles = (int32_t)((len + kTile - 1) / kTile);
-    const int32_t total = n_tiles * chunks;
-    Raw<T> next_w, next_r, next_u, next_delta, next_gate = {};
-    auto fetch_shared = [&](int32_t it) {
-        const int32_t tile = it / chunks;
-        const int n = (it - tile * chunks) * NC + threadIdx.x / LPC;
-        const int64_t t0 = (int64_t)tile * kTile + (threadIdx.x % LPC) * kSteps, end = n < p.N ? len : 0;
-        next_w = load_raw<T>(write_rows + n * p.write_n, t0, end);
-        next_r = load_raw<T>(read_rows + n * p.read_n, t0, end);
+    const int32_t row_tiles = (int32_t)((len + kTile - 1) / kTile), first_tile = w.seg * p.seg_tiles;
+    const int32_t seg_end = first_tile + p.seg_tiles, n_tiles = row_tiles < seg_end ? row_tiles : seg_end;  // the last one, exclusive
+    const int32_t total = n_tiles > first_tile ? (n_tiles - first_tile) * chunks : 0;
+    float all_dt = 0.0f;
+    TileLoader<T, LPC, NC, WAVES> loader;
+    Raw<T> next_u, next_delta, next_gate = {};
+    auto fetch_shared = [&](int32_t tile, int chunk) {
+        loader.load(write_rows, p.write_n, read_rows, p.read_n, chunk * NC, p.N, (int64_t)tile * kTile, len);
     };
     auto fetch_rows = [&](int32_t tile) {
         const int64_t t0 = (int64_t)tile * kTile + c * kSteps;
         next_u = load_raw<T>(u_row, t0, mine);
         next_delta = load_raw<T>(delta_row, t0, mine);
-        if (gate_row) next_gate = load_raw<T>(gate_row, t0, mine);
-    };
-    auto put_shared = [&](Tile& t) {
-        float f[kSteps];
-        widen_raw(next_w, f);
-        t.put(0, f);
-        widen_raw(next_r, f);
-        t.put(1, f);
+        if (!ENDS && gate_row) next_gate = load_raw<T>(gate_row, t0, mine);
     };
     if (total) {
-        fetch_shared(0);
-        fetch_rows(0);
-        put_shared(tiles[0]);
+        fetch_shared(first_tile, 0);
+        fetch_rows(first_tile);
+        loader.put(tiles[0]);
     }
     __syncthreads();
 
     float dt[kSteps], dtu[kSteps], y[kSteps], total_dt = 0.0f;
     Raw<T> gate_now = {};
     int32_t it = 0;
-    for (int32_t tile = 0; tile < n_tiles; ++tile) {
+    for (int32_t tile = first_tile; tile < n_tiles; ++tile) {
         const int64_t t0 = (int64_t)tile * kTile + c * kSteps;
+        const bool ragged = (int64_t)(tile + 1) * kTile > len;  // the row's last tile
         {
             float u[kSteps];
             widen_raw(next_u, u);
             widen_raw(next_delta, dt);
             gate_now = next_gate;
+            steps_of(dt, bias, p.flags, ragged, ragged ? steps_left(mine, t0) : kSteps);
             total_dt = 0.0f;
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
-                float v = dt[k] + bias;
-                if (p.flags & FMSELECTIVE_SOFTPLUS) v = softplus(v);
-                dt[k] = t0 + k < mine ? v : 0.0f;  // a step of length zero leaves the state as it is
                 dtu[k] = dt[k] * u[k];
                 y[k] = skip * u[k];
                 total_dt += dt[k];
             }
             if (tile + 1 < n_tiles) fetch_rows(tile + 1);
         }
+        if (ENDS) all_dt += total_dt;
+        if (LPC == 16 && !ENDS && marks && valid) {
+            float* mark = marks + (row * p.marks + tile) * p.N;
+            for (int n = c; n < p.N; n += LPC) mark[n] = held[n].y;
+        }
         for (int chunk = 0; chunk < chunks; ++chunk, ++it) {
-            if (it + 1 < total) fetch_shared(it + 1);
-            const Tile& now = tiles[it & 1];
-            const int n0 = chunk * NC, n_end = padded - n0 < NC ? padded - n0 : NC;
-            for (int nl = 0; nl < n_end; nl += 2) {
-                float a[2][kSteps], v[2][kSteps], P[2], S[2], enter[2];
+            if (it + 1 < total) fetch_shared(chunk + 1 < chunks ? tile : tile + 1, chunk + 1 < chunks ? chunk + 1 : 0);
+            const int n0 = chunk * NC, n_end = p.N - n0 < NC ? p.N - n0 : NC;
+            const float* at = tiles[it & 1].v[0][0][0][c];
+            float2* state = held + n0;
+            for (int n = 0; n < n_end; ++n, at += 8 * LPC, ++state) {
+                float a[kSteps], v[kSteps], r[kSteps];
+                const float2 e = *state;
+                steps_at<LPC>(at, v);
+                if (!ENDS) steps_at<LPC>(at + NC * 8 * LPC, r);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const float2 e = held[ch * stride + n0 + nl + q];
-                    enter[q] = e.y;
-                    now.get(0, nl + q, c, v[q]);
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        a[q][k] = exp2_fast(dt[k] * e.x);
-                        v[q][k] *= dtu[k];
-                    }
-                    S[q] = v[q][0];
-#pragma unroll
-                    for (int k = 1; k < kSteps; ++k) S[q] = __builtin_fmaf(a[q][k], S[q], v[q][k]);
-                    P[q] = exp2_fast(total_dt * e.x);
+                for (int k = 0; k < kSteps; ++k) {
+                    a[k] = exp2_fast(dt[k] * e.x);
+                    v[k] *= dtu[k];
                 }
-                scan_up<LPC>(P[0], S[0], P[1], S[1]);
+                float S = v[0], P = exp2_fast(total_dt * e.x);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    constexpr int kShift = LPC == 16 ? kRowShr1 : fmscan::kWaveShr1;
-                    float h = __builtin_fmaf(fmscan::dpp<kShift>(1.0f, P[q]), enter[q], fmscan::dpp<kShift>(0.0f, S[q]));
-                    const int n = n0 + nl + q;
-                    if (c == LPC - 1) held[ch * stride + n].y = __builtin_fmaf(P[q], enter[q], S[q]);
-                    if (marks && (c & 15) == 0) {
-                        const int32_t mark = tile * (LPC / 16) + c / 16;
-                        if (valid && n < p.N && mark < p.marks) marks[(row * p.marks + mark) * p.N + n] = h;
-                    }
-                    float r[kSteps];
-                    now.get(1, nl + q, c, r);
+                for (int k = 1; k < kSteps; ++k) S = __builtin_fmaf(a[k], S, v[k]);
+                scan_up<LPC>(P, S);
+                constexpr int kShift = LPC == 16 ? kRowShr1 : fmscan::kWaveShr1;
+                float h = __builtin_fmaf(fmscan::dpp<kShift>(1.0f, P), e.y, fmscan::dpp<kShift>(0.0f, S));
+                if (c == LPC - 1) state->y = __builtin_fmaf(P, e.y, S);
+                if (ENDS) continue;
+                if (LPC == 64 && marks && (c & 15) == 0) {
+                    const int32_t mark = tile * (LPC / 16) + c / 16;
+                    if (valid && mark < p.marks) marks[(row * p.marks + mark) * p.N + n0 + n] = h;
+                }
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        h = __builtin_fmaf(a[q][k], h, v[q][k]);
-                        y[k] = __builtin_fmaf(r[k], h, y[k]);
-                    }
+                for (int k = 0; k < kSteps; ++k) {
+                    h = __builtin_fmaf(a[k], h, v[k]);
+                    y[k] = __builtin_fmaf(r[k], h, y[k]);
                 }
             }
-            if (it + 1 < total) put_shared(tiles[(it + 1) & 1]);
+            if (it + 1 < total) loader.put(tiles[(it + 1) & 1]);
             __syncthreads();
         }
+        if (ENDS) continue;
         if (gate_row) {
             float z[kSteps];
             widen_raw(gate_now, z);
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) y[k] *= z[k] * sigmoid(z[k]);
         }
+        if (ragged) {
+            const int left = steps_left(mine, t0);
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) y[k] = t0 + k < mine ? y[k] : 0.0f;
+            for (int k = 0; k < kSteps; ++k) y[k] = k < left ? y[k] : 0.0f;
+        }
         if (valid) store_values<T, kSteps>(out + row * p.L, t0, p.L, y);
+    }
+    if constexpr (ENDS) {
+        // (the total's decay in one exponential of the summed steps, as within a tile)
+        all_dt = row_sum(all_dt);
+        if constexpr (LPC == 64)
+            all_dt = fmscan::lane_value(all_dt, 15) + fmscan::lane_value(all_dt, 31) + fmscan::lane_value(all_dt, 47) +
+                     fmscan::lane_value(all_dt, 63);
+        else
+            all_dt = __shfl(all_dt, lane | 15);
+        if (valid)
+            for (int n = c; n < p.N; n += LPC)
+                p.pairs[((int64_t)w.seg * p.rows + row) * p.N + n] = make_float2(exp2_fast(all_dt * held[n].x), held[n].y);
+        return;
     }
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) y[k] = 0.0f;
-    if (valid)
-        for (int64_t t0 = (int64_t)n_tiles * kTile + c * kSteps; t0 < p.L; t0 += kTile) store_values<T, kSteps>(out + row * p.L, t0, p.L, y);
-    if (final_state)
-        each_state([&](float2& e, int64_t r, int n) {
-            if (r >= 0) final_state[r * p.N + n] = e.y;
-        });
-}
-
-// Adds the values of the four rows of a wave and deals the sums out: of v[0..7] and v[8..15], row 0 gets the sums
-// of v[0..3], row 1 v[4..7], row 2 v[8..11], row 3 v[12..15]. Each swap exchanges halves of two registers, so one
-// addition settles both: 24 instructions for 16 sums.
-__device__ __forceinline__ float4 sum_rows(const float (&v)[16]) {
-    float w[8], x[4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const auto s = __builtin_amdgcn_permlane32_swap(f2u(v[i]), f2u(v[i + 8]), false, false);
-        w[i] = u2f(s[0]) + u2f(s[1]);
+    if (valid) {
+        const int64_t end = (int64_t)seg_end * kTile < p.L ? (int64_t)seg_end * kTile : p.L;
+        for (int64_t t0 = (int64_t)(n_tiles > first_tile ? n_tiles : first_tile) * kTile + c * kSteps; t0 < end; t0 += kTile)
+            store_values<T, kSteps>(out + row * p.L, t0, p.L, y);
+        if (final_state && w.seg == p.segments - 1)
+            for (int n = c; n < p.N; n += LPC) final_state[row * p.N + n] = held[n].y;
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const auto s = __builtin_amdgcn_permlane16_swap(f2u(w[i]), f2u(w[i + 4]), false, false);
-        x[i] = u2f(s[0]) + u2f(s[1]);
-    }
-    return make_float4(x[0], x[1], x[2], x[3]);
 }
 
 struct ScanGrads {
@@ -338,9 +402,13 @@ struct ScanGrads {
     float *shared_part;                  // [block][n][mark][256]: sums of write's and read's gradients over the block's channels
 };
 
+// LDS of the backward kernel: the shared tile, the waves' sums of two states (twice: one being read), and per
+// channel and state A log2 e, the gradient that arrives from later steps, the sum for dA, the state before the tile
 template <int WAVES>
+constexpr size_t scan_sums_bytes() { return (size_t)2 * WAVES * 2 * 256 * sizeof(float); }
+template <int WAVES, int R>
 size_t scan_backward_lds(int N) {
-    return scan_tiles_bytes<16, WAVES>() + sizeof(float4) * 2 * WAVES * 2 * 64 + (size_t)WAVES * 4 * state_stride(N) * sizeof(float4);
+    return sizeof(SharedTile<16, 16>) + scan_sums_bytes<WAVES>() + (size_t)WAVES * R * 4 * state_stride(N) * sizeof(float4);
 }
 
 // Backward. The tiles are walked from the last to the first. In a tile the states are made again from the state that
@@ -349,241 +417,289 @@ size_t scan_backward_lds(int N) {
 //   dtokens = dt sum_n dh write + skip g      dA = sum_t dt p      p = dh a h[t-1]
 //   ddt = u sum_n dh write + sum_n A p        dwrite = sum_d dh dt u      dread = sum_d g h
 // The sums over n stay in registers, those over time are added up in LDS, one float a state and channel. The sums
-// over the channels are made in the wave (its 4 channels, sum_rows), over the block's waves in LDS and over
-// the blocks by a second kernel, always in the same order.
-template <typename T, int WAVES>
+// over the channels are made in the lane (its R sets of channels), in the wave (4 channels side by side), over the
+// block's waves in LDS and over the blocks by a second kernel, always in the same order.
+// Rows that are too few to fill the GPU are cut into segments, as in forward: the first launch (ENDS) finds what each
+// segment but the first hands on of a gradient that enters it from behind.
+template <typename T, int WAVES, int R, bool ENDS>
 __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, ScanGrads o) {
-    constexpr int LPC = 16, kTile = LPC * kSteps, CW = 4;
-    using Tile = SharedTile<LPC, WAVES>;
-    constexpr int NC = Tile::kStates;
-    extern __shared__ char lds[];
-    Tile* tiles = reinterpret_cast<Tile*>(lds);
-    float4* sums = reinterpret_cast<float4*>(lds + scan_tiles_bytes<LPC, WAVES>());  // [parity][wave][state of the pair][lane]
+    constexpr int LPC = 16, NC = 16, kTile = LPC * kSteps;
+    using Tile = SharedTile<LPC, NC>;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    Tile& shared = *reinterpret_cast<Tile*>(lds);
+    float* sums = reinterpret_cast<float*>(lds + sizeof(Tile));  // [parity][wave][state of the pair][256]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, ch = lane >> 4;
-    const int stride = state_stride(p.N);
-    // per channel and state: A log2 e, the gradient that arrives from later steps, the sum for dA, the state before the tile
-    float4* held = sums + 2 * WAVES * 2 * 64 + wave * CW * stride;
 
-    const uint32_t bg = blockIdx.x / (uint32_t)p.blocks_per_group, block = blockIdx.x - bg * p.blocks_per_group;
-    const uint32_t b = bg / (uint32_t)p.G, g = bg - b * p.G;
-    const int32_t first = (int32_t)(block * WAVES + wave) * CW, local = first + ch;
-    const bool valid = local < p.per_group;
-    const int32_t d = (int32_t)g * p.per_group + (valid ? local : p.per_group - 1);
-    const int64_t row = (int64_t)b * p.D + d;
-    const int64_t len = row_length(p.lengths, b, p.L), mine = valid ? len : 0;
-    const T* u_row = (const T*)p.tokens + b * p.tokens_b + d * p.tokens_d;
-    const T* delta_row = (const T*)p.delta + b * p.delta_b + d * p.delta_d;
-    const T* gate_row = p.gate ? (const T*)p.gate + b * p.gate_b + d * p.gate_d : nullptr;
-    const T* dy_row = (const T*)o.out_grad + b * o.out_b + d * o.out_d;
+    const Place at = place_of(p);
+    const uint32_t b = at.b, g = at.g;
+    const int32_t local = (int32_t)(at.block * WAVES + wave) * 4 * R + ch;  // the lane's first channel; the others follow by fours
+    const int32_t d0 = (int32_t)g * p.per_group + local;
+    const int64_t len = row_length(p.lengths, b, p.L);
+    bool valid[R];
+    int64_t mine[R];
+    float skip[R], bias[R], skip_sum[R], bias_sum[R], all_dt = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        valid[r] = local + 4 * r < p.per_group;
+        mine[r] = valid[r] ? len : 0;
+        const int32_t d = valid[r] ? d0 + 4 * r : (int32_t)p.D - 1;
+        skip[r] = p.skip ? param<T>(p.skip, d, p.flags & FMSELECTIVE_NARROW_SKIP) : 0.0f;
+        bias[r] = p.delta_bias ? param<T>(p.delta_bias, d, p.flags & FMSELECTIVE_NARROW_BIAS) : 0.0f;
+        skip_sum[r] = bias_sum[r] = 0.0f;
+    }
+    // (a row beyond the group is addressed but, with no steps that count, never read)
+    const int64_t row = (int64_t)b * p.D + d0;
+    const T* u_row = (const T*)p.tokens + b * p.tokens_b + d0 * p.tokens_d;
+    const T* delta_row = (const T*)p.delta + b * p.delta_b + d0 * p.delta_d;
+    const T* gate_row = p.gate ? (const T*)p.gate + b * p.gate_b + d0 * p.gate_d : nullptr;
+    const T* dy_row = (const T*)o.out_grad + b * o.out_b + d0 * o.out_d;
     const T* write_rows = (const T*)p.write + b * p.write_b + g * p.write_g;
     const T* read_rows = (const T*)p.read + b * p.read_b + g * p.read_g;
-    const float skip = p.skip ? param<T>(p.skip, d, p.flags & FMSELECTIVE_NARROW_SKIP) : 0.0f;
-    const float bias = p.delta_bias ? param<T>(p.delta_bias, d, p.flags & FMSELECTIVE_NARROW_BIAS) : 0.0f;
 
-    const int padded = padded_states(p.N);
-    auto each_state = [&](auto&& f) {
-        for (int i = lane; i < CW * padded; i += 64) {
-            const int k = i / padded, n = i - k * padded;
-            const bool real = n < p.N && first + k < p.per_group;
-            f(held[k * stride + n], real ? (int64_t)b * p.D + (int64_t)g * p.per_group + first + k : (int64_t)-1, n);
+    const int stride = state_stride(p.N);
+    float4* held = reinterpret_cast<float4*>(lds + sizeof(Tile) + scan_sums_bytes<WAVES>()) + (wave * 4 * R + ch) * stride;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        for (int n = c; n < p.N; n += LPC) {
+            float e = 0.0f, rate = 0.0f;
+            if (valid[r]) {
+                const int64_t at_n = (row + 4 * r) * p.N + n;
+                rate = p.A[(int64_t)(d0 + 4 * r) * p.N + n] * kLog2E;
+                if (!ENDS) {
+                    if (o.final_grad) e = o.final_grad[at_n];
+#pragma unroll 4
+                    for (int32_t j = p.segments - 1; j > at.seg; --j) {
+                        const float2 q = p.pairs[j * p.rows * p.N + at_n];
+                        e = __builtin_fmaf(q.x, e, q.y);
+                    }
+                }
+            }
+            held[4 * r * stride + n] = make_float4(rate, e, 0.0f, 0.0f);
         }
-    };
-    each_state([&](float4& e, int64_t r, int n) {
-        e.x = r < 0 ? 0.0f : p.A[(r - (int64_t)b * p.D) * p.N + n] * kLog2E;
-        e.y = r < 0 || !o.final_grad ? 0.0f : o.final_grad[r * p.N + n];
-        e.z = 0.0f;
-        e.w = 0.0f;
-    });
 
     const int chunks = (p.N + NC - 1) / NC;
-    const int32_t n_tiles = (int32_t)((len + kTile - 1) / kTile);
-    const int32_t total = n_tiles * chunks;
-    Raw<T> next_w, next_r;
-    auto fetch_shared = [&](int32_t it) {
-        const int32_t back = it / chunks;
-        const int n = (it - back * chunks) * NC + threadIdx.x / LPC;
-        const int64_t t0 = (int64_t)(n_tiles - 1 - back) * kTile + (threadIdx.x % LPC) * kSteps, end = n < p.N ? len : 0;
-        next_w = load_raw<T>(write_rows + n * p.write_n, t0, end);
-        next_r = load_raw<T>(read_rows + n * p.read_n, t0, end);
+    const int32_t row_tiles = (int32_t)((len + kTile - 1) / kTile), first_tile = at.seg * p.seg_tiles;
+    const int32_t seg_end = first_tile + p.seg_tiles, n_tiles = row_tiles < seg_end ? row_tiles : seg_end;
+    TileLoader<T, LPC, NC, WAVES> loader;
+    auto fetch_shared = [&](int32_t tile, int chunk) {
+        loader.load(write_rows, p.write_n, read_rows, p.read_n, chunk * NC, p.N, (int64_t)tile * kTile, len);
     };
-    auto put_shared = [&](Tile& t) {
-        float f[kSteps];
-        widen_raw(next_w, f);
-        t.put(0, f);
-        widen_raw(next_r, f);
-        t.put(1, f);
-    };
-    if (total) {
-        fetch_shared(0);
-        put_shared(tiles[0]);
-    }
-    __syncthreads();
+    if (n_tiles > first_tile) fetch_shared(n_tiles - 1, 0);
 
-    float skip_sum = 0.0f, bias_sum = 0.0f;
-    int32_t it = 0, pairs = 0;
-    float* part = o.shared_part + (int64_t)blockIdx.x * p.N * p.marks * 256;
-    for (int32_t tile = n_tiles - 1; tile >= 0; --tile) {
+    uint32_t parity = 0;
+    float* part = ENDS ? nullptr : o.shared_part + at.line * p.N * p.marks * 256;
+    for (int32_t tile = n_tiles - 1; tile >= first_tile; --tile) {
         const int64_t t0 = (int64_t)tile * kTile + c * kSteps;
-        float dt[kSteps], dtu[kSteps], gy[kSteps], sum_w[kSteps], sum_a[kSteps], y[kSteps], total_dt = 0.0f;
-        {
+        const bool ragged = (int64_t)(tile + 1) * kTile > len;
+        float dt[R][kSteps], dtu[R][kSteps], gy[R][kSteps], sum_w[R][kSteps], sum_a[R][kSteps], y[R][kSteps], total_dt[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const Raw<T> raw_d = load_raw<T>(delta_row + 4 * r * p.delta_d, t0, mine[r]),
+                         raw_g = load_raw<T>(dy_row + 4 * r * o.out_d, t0, mine[r]);
+            Raw<T> raw_u = {}, raw_z = {};
+            if (!ENDS) raw_u = load_raw<T>(u_row + 4 * r * p.tokens_d, t0, mine[r]);
+            if (gate_row) raw_z = load_raw<T>(gate_row + 4 * r * p.gate_d, t0, mine[r]);
+            if (!ENDS)
+                for (int n = c; n < p.N; n += LPC)
+                    held[4 * r * stride + n].w = valid[r] ? o.marks[((row + 4 * r) * p.marks + tile) * p.N + n] : 0.0f;
             float u[kSteps], z[kSteps];
-            load_values<T, kSteps>(u_row, t0, mine, u);
-            load_values<T, kSteps>(delta_row, t0, mine, dt);
-            load_values<T, kSteps>(dy_row, t0, mine, gy);
-            if (gate_row) load_values<T, kSteps>(gate_row, t0, mine, z);
+            widen_raw(raw_d, dt[r]);
+            widen_raw(raw_g, gy[r]);
+            steps_of(dt[r], bias[r], p.flags, ragged, ragged ? steps_left(mine[r], t0) : kSteps);
+            if (gate_row) {
+                widen_raw(raw_z, z);
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) gy[r][k] *= z[k] * sigmoid(z[k]);
+            }
+            widen_raw(raw_u, u);
+            total_dt[r] = 0.0f;
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
-                float v = dt[k] + bias;
-                if (p.flags & FMSELECTIVE_SOFTPLUS) v = softplus(v);
-                dt[k] = t0 + k < mine ? v : 0.0f;
-                dtu[k] = dt[k] * u[k];
-                total_dt += dt[k];
-                if (gate_row) gy[k] *= z[k] * sigmoid(z[k]);
-                sum_w[k] = sum_a[k] = y[k] = 0.0f;
+                dtu[r][k] = dt[r][k] * u[k];
+                total_dt[r] += dt[r][k];
+                sum_w[r][k] = sum_a[r][k] = y[r][k] = 0.0f;
             }
+            if (ENDS) all_dt += total_dt[r];
         }
-        each_state([&](float4& e, int64_t r, int n) { e.w = r < 0 ? 0.0f : o.marks[(r * p.marks + tile) * p.N + n]; });
-        __builtin_amdgcn_wave_barrier();  // what the wave's lanes have written its lanes read: LDS answers in order
-        for (int chunk = 0; chunk < chunks; ++chunk, ++it) {
-            if (it + 1 < total) fetch_shared(it + 1);
-            const Tile& now = tiles[it & 1];
-            const int n0 = chunk * NC, n_end = padded - n0 < NC ? padded - n0 : NC;
-            for (int nl = 0; nl < n_end; nl += 2, ++pairs) {
-                float a[2][kSteps], h[2][kSteps], m[2][kSteps], dh[2][kSteps], P[2], S[2], Q[2], R[2];
-                float4 e[2];
+        for (int chunk = 0; chunk < chunks; ++chunk) {
+            loader.put(shared);
+            if (chunk + 1 < chunks) fetch_shared(tile, chunk + 1);
+            else if (tile > first_tile) fetch_shared(tile - 1, 0);
+            __syncthreads();
+            const int n0 = chunk * NC, n_end = p.N - n0 < NC ? p.N - n0 : NC;
+            const float* steps = shared.v[0][0][0][c];
+            float4* state = held + n0;
+            for (int n = 0; n < n_end; ++n, steps += 8 * LPC, ++state) {
+                float w[kSteps], rd[kSteps];
+                if (!ENDS) steps_at<LPC>(steps, w);
+                steps_at<LPC>(steps + NC * 8 * LPC, rd);
+                float write_terms[kSteps], read_terms[kSteps];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    e[q] = held[ch * stride + n0 + nl + q];
-                    now.get(0, nl + q, c, h[q]);
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        a[q][k] = exp2_fast(dt[k] * e[q].x);
-                        h[q][k] *= dtu[k];
-                    }
-                    S[q] = h[q][0];
-#pragma unroll
-                    for (int k = 1; k < kSteps; ++k) S[q] = __builtin_fmaf(a[q][k], S[q], h[q][k]);
-                    P[q] = exp2_fast(total_dt * e[q].x);
-                    Q[q] = P[q];
-                    now.get(1, nl + q, c, dh[q]);
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) dh[q][k] *= gy[k];
-                    R[q] = dh[q][kSteps - 1];
-#pragma unroll
-                    for (int k = kSteps - 2; k >= 0; --k) R[q] = __builtin_fmaf(a[q][k + 1], R[q], dh[q][k]);
-                    R[q] *= a[q][0];
-                }
-                scan_up<16>(P[0], S[0], P[1], S[1]);
-                scan_down(Q[0], R[0], Q[1], R[1]);
-                float4 rows[2];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    float s = __builtin_fmaf(fmscan::dpp<kRowShr1>(1.0f, P[q]), e[q].w, fmscan::dpp<kRowShr1>(0.0f, S[q]));
+                for (int r = 0; r < R; ++r) {
+                    float4& mem = state[4 * r * stride];
+                    const float4 e = mem;
+                    float a[kSteps], h[kSteps], dh[kSteps];
 #pragma unroll
                     for (int k = 0; k < kSteps; ++k) {
-                        m[q][k] = a[q][k] * s;
-                        s = h[q][k] = m[q][k] + h[q][k];
+                        a[k] = exp2_fast(dt[r][k] * e.x);
+                        dh[k] = rd[k] * gy[r][k];
+                        if (!ENDS) h[k] = w[k] * dtu[r][k];
                     }
-                    if (gate_row) {
-                        float r[kSteps];
-                        now.get(1, nl + q, c, r);
+                    float S = 0.0f, P = exp2_fast(total_dt[r] * e.x), D = dh[kSteps - 1], Q = P;
 #pragma unroll
-                        for (int k = 0; k < kSteps; ++k) y[k] = __builtin_fmaf(r[k], h[q][k], y[k]);
+                    for (int k = kSteps - 1; k > 0; --k) D = __builtin_fmaf(a[k], D, dh[k - 1]);
+                    D *= a[0];
+                    if constexpr (ENDS) {
+                        scan_down(Q, D);
+                        if (c == 0) mem.y = __builtin_fmaf(Q, e.y, D);
+                        continue;
                     }
-                    float t = __builtin_fmaf(fmscan::dpp<fmscan::kRowShl1>(1.0f, Q[q]), e[q].y,
-                                             fmscan::dpp<fmscan::kRowShl1>(0.0f, R[q]));
-                    float& arriving = held[ch * stride + n0 + nl + q].y;
-                    if (c == 0) arriving = __builtin_fmaf(Q[q], e[q].y, R[q]);
+                    S = h[0];
+#pragma unroll
+                    for (int k = 1; k < kSteps; ++k) S = __builtin_fmaf(a[k], S, h[k]);
+                    scan_both(P, S, Q, D);
+                    const float enter = __builtin_fmaf(fmscan::dpp<kRowShr1>(1.0f, P), e.w, fmscan::dpp<kRowShr1>(0.0f, S));
+                    float back = __builtin_fmaf(fmscan::dpp<fmscan::kRowShl1>(1.0f, Q), e.y, fmscan::dpp<fmscan::kRowShl1>(0.0f, D));
+                    if (c == 0) mem.y = __builtin_fmaf(Q, e.y, D);
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) {
+                        h[k] = __builtin_fmaf(a[k], k ? h[k - 1] : enter, h[k]);
+                        y[r][k] = __builtin_fmaf(rd[k], h[k], y[r][k]);
+                        read_terms[k] = r ? __builtin_fmaf(gy[r][k], h[k], read_terms[k]) : gy[r][k] * h[k];
+                    }
+                    float in_time = 0.0f;
 #pragma unroll
                     for (int k = kSteps - 1; k >= 0; --k) {
-                        dh[q][k] += t;
-                        t = a[q][k] * dh[q][k];
-                    }
-                    float w[kSteps], v[16], in_time = 0.0f;
-                    now.get(0, nl + q, c, w);
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        sum_w[k] = __builtin_fmaf(dh[q][k], w[k], sum_w[k]);
-                        v[k] = dh[q][k] * dtu[k];
-                        v[8 + k] = gy[k] * h[q][k];
-                        const float pk = dh[q][k] * m[q][k];
-                        sum_a[k] = __builtin_fmaf(e[q].x, pk, sum_a[k]);
-                        in_time = __builtin_fmaf(dt[k], pk, in_time);
+                        dh[k] += back;
+                        back = a[k] * dh[k];
+                        const float pk = back * (k ? h[k - 1] : enter);
+                        sum_w[r][k] = __builtin_fmaf(dh[k], w[k], sum_w[r][k]);
+                        sum_a[r][k] = __builtin_fmaf(e.x, pk, sum_a[r][k]);
+                        in_time = __builtin_fmaf(dt[r][k], pk, in_time);
+                        write_terms[k] = r ? __builtin_fmaf(dh[k], dtu[r][k], write_terms[k]) : dh[k] * dtu[r][k];
                     }
                     in_time = row_sum(in_time);
-                    if (c == 15) held[ch * stride + n0 + nl + q].z = e[q].z + in_time;
-                    rows[q] = sum_rows(v);
+                    if (c == 15) mem.z = e.z + in_time;
                 }
-                float4* mine_sums = sums + (pairs & 1) * WAVES * 2 * 64;
-                mine_sums[(wave * 2 + 0) * 64 + lane] = rows[0];
-                mine_sums[(wave * 2 + 1) * 64 + lane] = rows[1];
-                __syncthreads();
-                // two states' 64 float4 each, over the waves: the first two waves of the block add one each
-                if (wave < 2) {
-                    const int n = n0 + nl + wave;
-                    float4 s = mine_sums[wave * 64 + lane];
-#pragma unroll
-                    for (int w = 1; w < WAVES; ++w) {
-                        const float4 v = mine_sums[(w * 2 + wave) * 64 + lane];
-                        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-                    }
-                    if (n < p.N) reinterpret_cast<float4*>(part + ((int64_t)n * p.marks + tile) * 256)[lane] = s;
-                }
-            }
-            if (it + 1 < total) put_shared(tiles[(it + 1) & 1]);
-            __syncthreads();
-        }
-        {
-            float u[kSteps], dd[kSteps], x[kSteps], z[kSteps];
-            load_values<T, kSteps>(u_row, t0, mine, u);
-            load_values<T, kSteps>(delta_row, t0, mine, x);
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                float v = __builtin_fmaf(u[k], sum_w[k], kLn2 * sum_a[k]);
-                if (p.flags & FMSELECTIVE_SOFTPLUS) v *= sigmoid(x[k] + bias);
-                const bool in = t0 + k < mine;
-                dd[k] = in ? v : 0.0f;
-                bias_sum += dd[k];
-                skip_sum = __builtin_fmaf(gy[k], u[k], skip_sum);
-                x[k] = in ? __builtin_fmaf(dt[k], sum_w[k], skip * gy[k]) : 0.0f;
-                y[k] = __builtin_fmaf(skip, u[k], y[k]);
-            }
-            if (valid) {
-                store_values<T, kSteps>((T*)o.tokens + row * p.L, t0, p.L, x);
-                store_values<T, kSteps>((T*)o.delta + row * p.L, t0, p.L, dd);
-            }
-            if (gate_row) {
-                load_values<T, kSteps>(dy_row, t0, mine, dd);
-                load_values<T, kSteps>(gate_row, t0, mine, z);
+                if constexpr (ENDS) continue;
+                // The 4 channels side by side: a swap exchanges halves of two registers, so that one addition settles
+                // both. First the halves of the wave (lanes below 32 keep write's sums, the others read's), then
+                // the rows of a half (the even one keeps steps 0 to 3, the odd one 4 to 7).
+                float half[kSteps];
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
-                    const float v = dd[k] * y[k] * silu_slope(z[k], sigmoid(z[k]));
-                    dd[k] = t0 + k < mine ? v : 0.0f;
+                    const auto s = __builtin_amdgcn_permlane32_swap(f2u(write_terms[k]), f2u(read_terms[k]), false, false);
+                    half[k] = u2f(s[0]) + u2f(s[1]);
                 }
-                if (valid) store_values<T, kSteps>((T*)o.gate + row * p.L, t0, p.L, dd);
+                float4 row_sums;
+                float* q = &row_sums.x;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const auto s = __builtin_amdgcn_permlane16_swap(f2u(half[k]), f2u(half[k + 4]), false, false);
+                    q[k] = u2f(s[0]) + u2f(s[1]);
+                }
+                reinterpret_cast<float4*>(sums + ((parity * WAVES + wave) * 2 + (n & 1)) * 256)[lane] = row_sums;
+                if ((n & 1) || n + 1 == n_end) {
+                    // two states (or the last one): their 512 sums over the waves, dealt to all threads
+                    __syncthreads();
+                    constexpr int V = 512 / (64 * WAVES);
+                    const int f = threadIdx.x * V, n_first = n0 + (n & ~1);
+                    if (n_first + f / 256 <= n0 + n) {
+                        float total[V];
+                        const float* from = sums + parity * WAVES * 512 + f;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) total[i] = from[i];
+#pragma unroll
+                        for (int v = 1; v < WAVES; ++v)
+#pragma unroll
+                            for (int i = 0; i < V; ++i) total[i] += from[v * 512 + i];
+                        float* to = part + ((int64_t)(n_first + f / 256) * p.marks + tile) * 256 + f % 256;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) to[i] = total[i];
+                    }
+                    parity ^= 1;
+                }
+            }
+            __syncthreads();  // the tile may be filled again
+        }
+        if (ENDS) continue;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t at_row = (row + 4 * r) * p.L;
+            const int left = ragged ? steps_left(mine[r], t0) : kSteps;
+            float u[kSteps], dd[kSteps], x[kSteps], z[kSteps];
+            load_values<T, kSteps>(u_row + 4 * r * p.tokens_d, t0, mine[r], u);
+            load_values<T, kSteps>(delta_row + 4 * r * p.delta_d, t0, mine[r], x);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                dd[k] = __builtin_fmaf(u[k], sum_w[r][k], kLn2 * sum_a[r][k]);
+                if (p.flags & FMSELECTIVE_SOFTPLUS) dd[k] *= sigmoid(x[k] + bias[r]);
+                x[k] = __builtin_fmaf(dt[r][k], sum_w[r][k], skip[r] * gy[r][k]);
+                y[r][k] = __builtin_fmaf(skip[r], u[k], y[r][k]);
+            }
+            if (ragged) {
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    dd[k] = k < left ? dd[k] : 0.0f;
+                    x[k] = k < left ? x[k] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                bias_sum[r] += dd[k];
+                skip_sum[r] = __builtin_fmaf(gy[r][k], u[k], skip_sum[r]);
+            }
+            if (valid[r]) {
+                store_values<T, kSteps>((T*)o.tokens + at_row, t0, p.L, x);
+                store_values<T, kSteps>((T*)o.delta + at_row, t0, p.L, dd);
+            }
+            if (gate_row) {
+                load_values<T, kSteps>(dy_row + 4 * r * o.out_d, t0, mine[r], dd);
+                load_values<T, kSteps>(gate_row + 4 * r * p.gate_d, t0, mine[r], z);
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) dd[k] *= y[r][k] * silu_slope(z[k], sigmoid(z[k]));
+                if (ragged) {
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) dd[k] = k < left ? dd[k] : 0.0f;
+                }
+                if (valid[r]) store_values<T, kSteps>((T*)o.gate + at_row, t0, p.L, dd);
             }
         }
+    }
+    if constexpr (ENDS) {
+        static_assert(!ENDS || R == 1, "one set of channels");
+        all_dt = __shfl(row_sum(all_dt), lane | 15);
+        if (valid[0])
+            for (int n = c; n < p.N; n += LPC)
+                p.pairs[((int64_t)at.seg * p.rows + row) * p.N + n] = make_float2(exp2_fast(all_dt * held[n].x), held[n].y);
+        return;
     }
     float zero[kSteps];
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) zero[k] = 0.0f;
-    if (valid)
-        for (int64_t t0 = (int64_t)n_tiles * kTile + c * kSteps; t0 < p.L; t0 += kTile) {
-            store_values<T, kSteps>((T*)o.tokens + row * p.L, t0, p.L, zero);
-            store_values<T, kSteps>((T*)o.delta + row * p.L, t0, p.L, zero);
-            if (gate_row) store_values<T, kSteps>((T*)o.gate + row * p.L, t0, p.L, zero);
+    const int64_t end = (int64_t)seg_end * kTile < p.L ? (int64_t)seg_end * kTile : p.L;
+    const int64_t part_row = (int64_t)at.seg * p.rows + row;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        skip_sum[r] = row_sum(skip_sum[r]);
+        bias_sum[r] = row_sum(bias_sum[r]);
+        if (!valid[r]) continue;
+        const int64_t at_row = (row + 4 * r) * p.L;
+        for (int64_t t0 = (int64_t)(n_tiles > first_tile ? n_tiles : first_tile) * kTile + c * kSteps; t0 < end; t0 += kTile) {
+            store_values<T, kSteps>((T*)o.tokens + at_row, t0, p.L, zero);
+            store_values<T, kSteps>((T*)o.delta + at_row, t0, p.L, zero);
+            if (gate_row) store_values<T, kSteps>((T*)o.gate + at_row, t0, p.L, zero);
         }
-    skip_sum = row_sum(skip_sum);
-    bias_sum = row_sum(bias_sum);
-    if (valid && c == 15) {
-        if (o.skip_part) o.skip_part[row] = skip_sum;
-        if (o.bias_part) o.bias_part[row] = bias_sum;
+        if (c == 15) {
+            if (o.skip_part) o.skip_part[part_row + 4 * r] = skip_sum[r];
+            if (o.bias_part) o.bias_part[part_row + 4 * r] = bias_sum[r];
+        }
+        for (int n = c; n < p.N; n += LPC) {
+            const float4 e = held[4 * r * stride + n];
+            o.A_part[(part_row + 4 * r) * p.N + n] = e.z;
+            if (o.initial && at.seg == 0) o.initial[(row + 4 * r) * p.N + n] = e.y;
+        }
     }
-    each_state([&](float4& e, int64_t r, int n) {
-        if (r < 0) return;
-        o.A_part[r * p.N + n] = e.z;
-        if (o.initial) o.initial[r * p.N + n] = e.y;
-    });
 }
 
 // The gradients of write and read: the blocks' sums added up in their order and rounded once. A wave a

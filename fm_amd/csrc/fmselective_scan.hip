@@ -6,35 +6,71 @@ using fmselective::Scan;
 
 namespace {
 
-// Lanes a channel: 16, so that a wave works on 4 channels, or all 64, where that leaves too few waves.
+// Lanes a channel: 16, so that a wave works on 4 channels, or all 64 where that leaves too few waves; and where
+// that is too few as well, the rows are cut.
 #ifndef FMSELECTIVE_FEW_WAVES
 #define FMSELECTIVE_FEW_WAVES 2048
 #endif
-int lanes_per_channel(const fmselective_scan_inputs& in) {
-    const int64_t waves = in.B * in.G * ((in.D / in.G + 3) / 4);
-    return waves >= FMSELECTIVE_FEW_WAVES || in.L <= 128 ? 16 : 64;
+#ifndef FMSELECTIVE_CUT_BELOW
+#define FMSELECTIVE_CUT_BELOW 1024
+#endif
+#ifndef FMSELECTIVE_CUT_WANT
+#define FMSELECTIVE_CUT_WANT 2048
+#endif
+#ifndef FMSELECTIVE_WAVES64
+#define FMSELECTIVE_WAVES64 8
+#endif
+struct ForwardPlan {
+    int lanes;
+    Cut cut;
+    size_t bytes;  // of the pairs between segments
+};
+ForwardPlan plan_forward(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) {
+    ForwardPlan f;
+    const int64_t waves = B * G * ((D / G + 3) / 4);
+    f.lanes = waves >= FMSELECTIVE_FEW_WAVES || L <= 128 ? 16 : 64;
+    const int64_t have = f.lanes == 16 ? waves : B * D, tile = f.lanes * fmselective::kSteps;
+    f.cut = cut_of((L + tile - 1) / tile, have, have < FMSELECTIVE_CUT_BELOW ? FMSELECTIVE_CUT_WANT : have);
+    f.bytes = f.cut.segments > 1 ? (size_t)(f.cut.segments - 1) * B * D * N * sizeof(float2) : 0;
+    return f;
 }
 
-template <typename T, int LPC>
-int launch_forward(const char* who, const fmselective_scan_inputs& in, void* out, float* final_state, float* marks, hipStream_t stream) {
-    constexpr int WAVES = fmselective::kScanWaves;
-    const Scan p = scan_of(in, WAVES * 64 / LPC);
-    const int64_t blocks = in.B * in.G * p.blocks_per_group;
+template <typename T, int LPC, int WAVES>
+int launch_forward(const char* who, const fmselective_scan_inputs& in, Cut cut, void* out, float* final_state, float* marks,
+                   void* pairs, hipStream_t stream) {
+    const Scan p = scan_of(in, WAVES * 64 / LPC, cut, pairs);
+    const int64_t blocks = in.B * in.G * p.blocks_per_group * cut.segments;
     if (blocks > INT32_MAX) return fail(FMSCAN_E_SHAPE, "%s: B * D is too large for one launch", who);
-    static std::atomic<uint64_t> armed{0};
+    static std::atomic<uint64_t> armed{0}, armed_ends{0};
     const size_t lds = fmselective::scan_forward_lds<LPC, WAVES>(p.N);
-    const auto kernel = fmselective::selective_forward_kernel<T, LPC, WAVES>;
-    if (lds > 64 * 1024)
+    const auto kernel = fmselective::selective_forward_kernel<T, LPC, WAVES, false>;
+    const auto ends = fmselective::selective_forward_kernel<T, LPC, WAVES, true>;
+    if (lds > 64 * 1024) {
         if (int rc = raise_lds_limit((const void*)kernel, armed, who)) return rc;
+        if (int rc = raise_lds_limit((const void*)ends, armed_ends, who)) return rc;
+    }
+    if (cut.segments > 1) {
+        Scan q = p;  // every segment but the last
+        q.segments = cut.segments - 1;
+        ends<<<(unsigned)(blocks / cut.segments * q.segments), 64 * WAVES, lds, stream>>>(q, (T*)nullptr, nullptr, nullptr);
+        if (int rc = launched("selective scan (ends of segments)")) return rc;
+    }
     kernel<<<(unsigned)blocks, 64 * WAVES, lds, stream>>>(p, (T*)out, final_state, marks);
     return launched("selective scan (forward)");
 }
 
 }  // namespace
 
+namespace fmselective {
+namespace host {
+size_t forward_workspace_bytes(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) { return plan_forward(B, D, L, N, G).bytes; }
+}  // namespace host
+}  // namespace fmselective
+
 extern "C" {
 
-int fmselective_scan_forward(const fmselective_scan_inputs* in, void* out, float* final_state, float* marks, void* stream) {
+int fmselective_scan_forward(const fmselective_scan_inputs* in, void* out, float* final_state, float* marks, void* workspace,
+                             size_t workspace_bytes, void* stream) {
     const char* who = "fmselective_scan_forward";
     if (int rc = check_scan(who, in, kScanFlags)) return rc;
     if (!out) return fail(FMSCAN_E_NULL, "%s: out must not be NULL", who);
@@ -42,11 +78,24 @@ int fmselective_scan_forward(const fmselective_scan_inputs* in, void* out, float
     if (int rc = check_outputs(who, {{"out", out, in->B * in->D * in->L * esize_of(in->dtype)}, {"final_state", final_state, states},
                                      {"marks", marks, states * n_marks}}, input_ranges(*in)))
         return rc;
+    ForwardPlan f = plan_forward(in->B, in->D, in->L, in->N, in->G);
+    if (f.cut.segments > 1) {
+        if (!workspace || workspace_bytes < f.bytes || ((uintptr_t)workspace & 7u)) {
+            f.cut = {1, f.cut.segments * f.cut.seg_tiles};
+        } else if (int rc = check_outputs(who, {{"workspace", workspace, (int64_t)f.bytes}}, input_ranges(*in))) {
+            return rc;
+        } else if (int rc = check_alias(who, {{"workspace", workspace, (int64_t)f.bytes}},
+                                        {{"out", out, in->B * in->D * in->L * esize_of(in->dtype)}, {"final_state", final_state, states},
+                                         {"marks", marks, states * n_marks}})) {
+            return rc;
+        }
+    }
     int rc = 0;
     with_dtype(in->dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
-        rc = lanes_per_channel(*in) == 16 ? launch_forward<T, 16>(who, *in, out, final_state, marks, (hipStream_t)stream)
-                                          : launch_forward<T, 64>(who, *in, out, final_state, marks, (hipStream_t)stream);
+        constexpr int W = fmselective::kScanWaves;
+        rc = f.lanes == 16 ? launch_forward<T, 16, W>(who, *in, f.cut, out, final_state, marks, workspace, (hipStream_t)stream)
+                           : launch_forward<T, 64, FMSELECTIVE_WAVES64>(who, *in, f.cut, out, final_state, marks, workspace, (hipStream_t)stream);
     });
     return rc;
 }

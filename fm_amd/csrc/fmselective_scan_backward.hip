@@ -8,29 +8,57 @@ using fmselective::ScanGrads;
 namespace {
 
 constexpr int kBackWaves = fmselective::kScanWaves;
-constexpr int kBackChannels = 4 * kBackWaves;
 
+// Sets of channels a lane works on: two where that leaves two waves a SIMD, which halves the additions over
+// channels and the partial sums in memory; one otherwise, with the rows cut where those are too few.
+#ifndef FMSELECTIVE_BACK_TWO
+#define FMSELECTIVE_BACK_TWO 2048
+#endif
+#ifndef FMSELECTIVE_BACK_CUT_BELOW
+#define FMSELECTIVE_BACK_CUT_BELOW 1024
+#endif
+#ifndef FMSELECTIVE_BACK_CUT_WANT
+#define FMSELECTIVE_BACK_CUT_WANT 2048
+#endif
 struct BackPlan {
-    int64_t blocks, shared, states, rows;  // blocks; floats of the three kinds of partial sums
+    int sets;
+    Cut cut;
+    int64_t blocks, shared, states, rows, pairs;  // blocks; floats of the partial sums and of the pairs
+    size_t bytes() const { return (size_t)(shared + pairs + states + 2 * rows) * sizeof(float); }
 };
-BackPlan plan(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) {
+BackPlan plan_backward(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) {
     const int64_t per_group = D / G, marks = (L + fmselective::kMark - 1) / fmselective::kMark;
+    auto blocks = [&](int sets) { return B * G * ((per_group + 4 * kBackWaves * sets - 1) / (4 * kBackWaves * sets)); };
     BackPlan b;
-    b.blocks = B * G * ((per_group + kBackChannels - 1) / kBackChannels);
+    b.sets = blocks(2) * kBackWaves >= FMSELECTIVE_BACK_TWO ? 2 : 1;
+    b.blocks = blocks(b.sets);
+    const int64_t waves = b.blocks * kBackWaves;
+    b.cut = cut_of(marks, waves, waves < FMSELECTIVE_BACK_CUT_BELOW ? FMSELECTIVE_BACK_CUT_WANT : waves);
     b.shared = b.blocks * N * marks * 256;
-    b.states = B * D * N;
-    b.rows = B * D;
+    b.pairs = b.cut.segments > 1 ? 2 * b.cut.segments * B * D * N : 0;
+    b.states = b.cut.segments * B * D * N;
+    b.rows = b.cut.segments * B * D;
     return b;
+}
+
+template <typename T, int R, bool ENDS>
+int launch_backward(const char* who, const Scan& p, const ScanGrads& g, int64_t blocks, hipStream_t stream) {
+    static std::atomic<uint64_t> armed{0};
+    const size_t lds = fmselective::scan_backward_lds<kBackWaves, R>(p.N);
+    const auto kernel = fmselective::selective_backward_kernel<T, kBackWaves, R, ENDS>;
+    if (lds > 64 * 1024)
+        if (int rc = raise_lds_limit((const void*)kernel, armed, who)) return rc;
+    kernel<<<(unsigned)blocks, 64 * kBackWaves, lds, stream>>>(p, g);
+    return launched("selective scan (backward)");
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t fmselective_scan_workspace_bytes(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int dtype) {
+size_t fmselective_scan_workspace_bytes(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int dtype, int backward) {
     if (check_states("fmselective_scan_workspace_bytes", B, D, L, N, G, dtype)) return 0;
-    const BackPlan b = plan(B, D, L, N, G);
-    return (size_t)(b.shared + b.states + 2 * b.rows) * sizeof(float);
+    return backward ? plan_backward(B, D, L, N, G).bytes() : forward_workspace_bytes(B, D, L, N, G);
 }
 
 int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselective_scan_grads* grads, void* workspace,
@@ -45,13 +73,13 @@ int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselecti
                     "delta_bias where they are", who);
     for (int i = 0; i < 2; ++i)
         if (int rc = check_stride(who, "out_grad", o.out_grad_strides[i])) return rc;
-    const BackPlan b = plan(in->B, in->D, in->L, in->N, in->G);
-    const size_t need = fmselective_scan_workspace_bytes(in->B, in->D, in->L, in->N, in->G, in->dtype);
+    const BackPlan b = plan_backward(in->B, in->D, in->L, in->N, in->G);
+    const size_t need = b.bytes();
     if (!workspace || workspace_bytes < need || !aligned16(workspace))
         return fail(FMSCAN_E_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed (got %zu)", who, need,
                     workspace ? workspace_bytes : (size_t)0);
     const int es = esize_of(in->dtype);
-    const int64_t seq = in->B * in->D * in->L * es, shared = in->B * in->G * in->N * in->L * es, states = b.states * 4;
+    const int64_t seq = in->B * in->D * in->L * es, shared = in->B * in->G * in->N * in->L * es, states = in->B * in->D * in->N * 4;
     const int64_t marks = states * ((in->L + fmselective::kMark - 1) / fmselective::kMark);
     const Range outs[] = {{"tokens' gradient", o.tokens, seq}, {"delta's gradient", o.delta, seq}, {"gate's gradient", o.gate, seq},
                           {"write's gradient", o.write, shared}, {"read's gradient", o.read, shared},
@@ -68,9 +96,10 @@ int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselecti
         for (const Range& q : outs)
             if (&q != &r && overlap(q, r)) return fail(FMSCAN_E_ALIAS, "%s: %s overlaps %s", who, r.name, q.name);
     }
-    const Scan p = scan_of(*in, kBackChannels);
-    const int64_t lines = in->B * in->G * in->N, waves = lines * p.marks;
-    if (b.blocks > INT32_MAX || waves > (int64_t)INT32_MAX * 4)
+    float* const pairs = (float*)workspace + b.shared;
+    const Scan p = scan_of(*in, 4 * kBackWaves * b.sets, b.cut, pairs);
+    const int64_t lines = in->B * in->G * in->N, waves = lines * p.marks, blocks = b.blocks * b.cut.segments;
+    if (blocks > INT32_MAX || waves > (int64_t)INT32_MAX * 4)
         return fail(FMSCAN_E_SHAPE, "%s: B * D or B * G * N * L is too large for one launch", who);
     float* part = (float*)workspace;
     ScanGrads g = {};
@@ -84,27 +113,25 @@ int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselecti
     g.gate = o.gate;
     g.initial = o.initial_state;
     g.shared_part = part;
-    g.A_part = part + b.shared;
-    g.skip_part = o.skip ? part + b.shared + b.states : nullptr;
-    g.bias_part = o.delta_bias ? part + b.shared + b.states + b.rows : nullptr;
+    g.A_part = pairs + b.pairs;
+    g.skip_part = o.skip ? g.A_part + b.states : nullptr;
+    g.bias_part = o.delta_bias ? g.A_part + b.states + b.rows : nullptr;
     int rc = 0;
     with_dtype(in->dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
-        static std::atomic<uint64_t> armed{0};
-        const size_t lds = fmselective::scan_backward_lds<kBackWaves>(p.N);
-        const auto kernel = fmselective::selective_backward_kernel<T, kBackWaves>;
-        if (lds > 64 * 1024 && (rc = raise_lds_limit((const void*)kernel, armed, who))) return;
-        kernel<<<(unsigned)b.blocks, 64 * kBackWaves, lds, (hipStream_t)stream>>>(p, g);
-        if ((rc = launched("selective scan (backward)"))) return;
+        const hipStream_t st = (hipStream_t)stream;
+        if (b.cut.segments > 1 && (rc = launch_backward<T, 1, true>(who, p, g, blocks, st))) return;
+        rc = b.sets == 2 ? launch_backward<T, 2, false>(who, p, g, blocks, st) : launch_backward<T, 1, false>(who, p, g, blocks, st);
+        if (rc) return;
         fmselective::selective_shared_grads_kernel<T><<<(unsigned)((waves + 3) / 4), 256, 0, (hipStream_t)stream>>>(
             part, (T*)o.write, (T*)o.read, in->lengths, in->L, waves, p.N, p.G, p.marks, p.blocks_per_group);
         rc = launched("selective scan (gradients of write and read)");
     });
     if (rc) return rc;
     launch_column_sums(in->dtype,
-                       {{g.A_part, o.A, in->B, in->D * in->N, 0, 0},
-                        {g.skip_part, o.skip, in->B, in->D, (in->flags & FMSELECTIVE_NARROW_SKIP) != 0, 0},
-                        {g.bias_part, o.delta_bias, in->B, in->D, (in->flags & FMSELECTIVE_NARROW_BIAS) != 0, 0}},
+                       {{g.A_part, o.A, in->B * b.cut.segments, in->D * in->N, 0, 0},
+                        {g.skip_part, o.skip, in->B * b.cut.segments, in->D, (in->flags & FMSELECTIVE_NARROW_SKIP) != 0, 0},
+                        {g.bias_part, o.delta_bias, in->B * b.cut.segments, in->D, (in->flags & FMSELECTIVE_NARROW_BIAS) != 0, 0}},
                        (hipStream_t)stream);
     return launched("selective scan (sums of the parameters' gradients)");
 }

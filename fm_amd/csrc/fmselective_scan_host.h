@@ -10,6 +10,9 @@ namespace host {
 constexpr unsigned kScanFlags = FMSELECTIVE_SOFTPLUS | FMSELECTIVE_NARROW_BIAS | FMSELECTIVE_NARROW_SKIP;
 static_assert(kMark == FMSELECTIVE_MARK, "the marks' distance is part of the interface");
 
+// Bytes of the pairs between a forward call's segments (fmselective_scan.hip)
+size_t forward_workspace_bytes(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G);
+
 inline int check_states(const char* who, int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int dtype) {
     if (int rc = check_sizes(who, B, D, L, dtype)) return rc;
     if (N < 1 || N > FMSELECTIVE_MAX_STATES)
@@ -35,7 +38,23 @@ inline int check_scan(const char* who, const fmselective_scan_inputs* in, unsign
     return 0;
 }
 
-inline Scan scan_of(const fmselective_scan_inputs& in, int channels_per_block) {
+// How a row is cut: `segments` of `seg_tiles` tiles
+struct Cut {
+    int32_t segments, seg_tiles;
+};
+// Enough segments for `want` waves where `waves` are there without, at least two tiles each: with one the first
+// launch would be as long as the row's.
+inline Cut cut_of(int64_t tiles, int64_t waves, int64_t want) {
+    int64_t n = (want + waves - 1) / waves;
+    if (n > tiles / 2) n = tiles / 2;
+    if (n < 1) n = 1;
+    Cut c;
+    c.seg_tiles = (int32_t)((tiles + n - 1) / n);
+    c.segments = (int32_t)((tiles + c.seg_tiles - 1) / c.seg_tiles);
+    return c;
+}
+
+inline Scan scan_of(const fmselective_scan_inputs& in, int channels_per_block, Cut cut, void* pairs) {
     Scan p = {};
     p.tokens = in.tokens; p.delta = in.delta; p.gate = in.gate; p.write = in.write; p.read = in.read;
     p.skip = in.skip; p.delta_bias = in.delta_bias; p.A = in.A; p.initial = in.initial_state; p.lengths = in.lengths;
@@ -50,6 +69,10 @@ inline Scan scan_of(const fmselective_scan_inputs& in, int channels_per_block) {
     p.blocks_per_group = (p.per_group + channels_per_block - 1) / channels_per_block;
     p.marks = (int32_t)((in.L + kMark - 1) / kMark);
     p.flags = in.flags;
+    p.segments = cut.segments;
+    p.seg_tiles = cut.seg_tiles;
+    p.rows = in.B * in.D;
+    p.pairs = (float2*)pairs;
     return p;
 }
 

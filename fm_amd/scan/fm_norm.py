@@ -14,45 +14,42 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .fm_scan import _dtype_code, _on_device, _on_gpu, _ptr, _raw, _require
+from .fm_scan import _ptr, _raw, _require
+from .fm_selective import _call, _dense, _gpu, _parameter, _tracked, _type_of
 
 __all__ = ["fm_norm", "fm_norm_quantized", "FM_Norm"]
 
 
 def _check(inputs, weight, residual, eps):
     """(rows, D, dtype code, flags)"""
-    _require(inputs.dim() >= 1 and weight.dim() == 1, "inputs must be (..., D) and weight (D,)")
-    dev, dtype, D = inputs.device, inputs.dtype, inputs.shape[-1]
-    _on_gpu("inputs", inputs, dev)
-    code = _dtype_code(inputs)
-    _require(inputs.is_contiguous(), "inputs must be contiguous")
-    _require(D <= _lib.SELECTIVE_MAX_NORM, f"the last axis must have at most {_lib.SELECTIVE_MAX_NORM} elements, got {D}")
-    _on_gpu("weight", weight, dev)
-    _require(weight.dtype == torch.float32 or weight.dtype == dtype,
-             f"weight has dtype {weight.dtype}, expected torch.float32 or {dtype}")
-    _require(weight.shape == (D,) and weight.is_contiguous(), f"weight must be a dense {(D,)}, got {tuple(weight.shape)}")
-    _require(eps >= 0, f"eps must be >= 0, got {eps}")
+    _gpu("inputs", inputs)
+    if inputs.dim() < 1 or weight.dim() != 1:
+        _require(False, "inputs must be (..., D) and weight (D,)")
+    shape, dtype, dev = inputs.shape, inputs.dtype, inputs.device
+    D = shape[-1]
+    code = _type_of(inputs)
+    if D > _lib.SELECTIVE_MAX_NORM:
+        _require(False, f"the last axis must have at most {_lib.SELECTIVE_MAX_NORM} elements, got {D}")
+    if not eps >= 0:
+        _require(False, f"eps must be >= 0, got {eps}")
+    _dense("inputs", inputs, shape, dtype, dev)
+    flags = _parameter("weight", weight, (D,), dtype, dev, _lib.SELECTIVE_NARROW_WEIGHT)
     if residual is not None:
-        _on_gpu("residual", residual, dev)
-        _require(residual.dtype == dtype, f"residual has dtype {residual.dtype}, expected {dtype}")
-        _require(residual.shape == inputs.shape, f"residual must be {tuple(inputs.shape)}, got {tuple(residual.shape)}")
-        _require(residual.is_contiguous(), "residual must be contiguous")
-    return inputs.numel() // D if D else 0, D, code, 0 if weight.dtype == torch.float32 else _lib.SELECTIVE_NARROW_WEIGHT
+        _dense("residual", residual, shape, dtype, dev)
+    return inputs.numel() // D if D else 0, D, code, flags
 
 
 def _forward(inputs, weight, residual, eps, save=False, quantized=False):
     """(out, residual_out or None, inv_rms or None, scales or None)"""
     rows, D, code, flags = _check(inputs, weight, residual, eps)
-    dev = inputs.device
-    out = torch.empty(inputs.shape, dtype=torch.float8_e4m3fn if quantized else inputs.dtype, device=dev)
-    stream_out = None if residual is None else torch.empty_like(inputs)
+    dev, shape = inputs.device, inputs.shape
+    out = torch.empty(shape, dtype=torch.float8_e4m3fn if quantized else inputs.dtype, device=dev)
+    stream_out = None if residual is None else torch.empty(shape, dtype=inputs.dtype, device=dev)
     inv_rms = torch.empty(rows, dtype=torch.float32, device=dev) if save else None
-    scales = torch.empty(inputs.shape[:-1], dtype=torch.float32, device=dev) if quantized else None
+    scales = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if quantized else None
     if rows:
-        with _on_device(dev):
-            _lib.check(_raw.fmselective_norm_forward(
-                inputs.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(stream_out), out.data_ptr(), _ptr(scales),
-                _ptr(inv_rms), rows, D, code, flags, float(eps), torch.cuda.current_stream(dev).cuda_stream))
+        _call(dev, _raw.fmselective_norm_forward, inputs.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(stream_out),
+              out.data_ptr(), _ptr(scales), _ptr(inv_rms), rows, D, code, flags, float(eps))
     elif quantized:
         scales.zero_()
     return out, stream_out, inv_rms, scales
@@ -87,11 +84,9 @@ class FM_Norm(torch.autograd.Function):
         residual_grad = None if residual_grad is None else residual_grad.contiguous()
         need = _raw.fmselective_norm_workspace_bytes(rows, D, code)
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        with _on_device(dev):
-            _lib.check(_raw.fmselective_norm_backward(
-                out_grad.data_ptr(), _ptr(residual_grad), stream_in.data_ptr(), weight.data_ptr(), inv_rms.data_ptr(),
-                grad.data_ptr(), d_weight.data_ptr(), rows, D, code, flags, workspace.data_ptr(), need,
-                torch.cuda.current_stream(dev).cuda_stream))
+        _call(dev, _raw.fmselective_norm_backward, out_grad.data_ptr(), _ptr(residual_grad), stream_in.data_ptr(),
+              weight.data_ptr(), inv_rms.data_ptr(), grad.data_ptr(), d_weight.data_ptr(), rows, D, code, flags,
+              workspace.data_ptr(), need)
         return grad, d_weight, grad if ctx.needs_input_grad[2] else None, None
 
 
@@ -107,7 +102,10 @@ def fm_norm(inputs, weight, residual=None, eps=1e-6):
     Returns (out (..., D), r (..., D)): r is the residual of the next block. What the norm sees is r as it is
     stored, rounded. Differentiable once, in inputs, weight and residual.
     """
-    out, stream_out = FM_Norm.apply(inputs, weight, residual, eps)
+    if _tracked(inputs, weight, residual):
+        out, stream_out = FM_Norm.apply(inputs, weight, residual, eps)
+    else:
+        out, stream_out, _, _ = _forward(inputs, weight, residual, eps)
     return out, (inputs if residual is None else stream_out)
 
 

@@ -11,87 +11,119 @@ implementation behind them. The reference has no counterpart of these operators.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .fm_scan import _dtype_code, _on_device, _on_gpu, _ptr, _raw, _require
+from .fm_scan import _DTYPES, _dtype_code, _on_gpu, _ptr, _raw, _require
 
 __all__ = ["fm_conv", "fm_conv_step", "FM_Conv", "fm_selective_scan", "fm_selective_step", "FM_Selective"]
 
 
-def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+# The checks come as one condition for the usual case and a function that says what is wrong: a call for one
+# token takes a few microseconds, and messages that are put together beforehand would double that.
+
+def _gpu(name, t):
+    if not t.is_cuda:
+        _on_gpu(name, t, t.device)
 
 
-def _sequence(name, t, shape, like):
-    """A (B, D, L) input: any batch and channel stride, time dense."""
-    _on_gpu(name, t, like.device)
-    _require(t.dtype == like.dtype, f"{name} has dtype {t.dtype}, expected {like.dtype}")
+def _wrong(name, t, shape, dtypes, dev, strides):
+    _require(t.device == dev, f"{name} is on {t.device}, expected {dev}")
+    _require(t.dtype in dtypes, f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
     _require(t.shape == shape, f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    _require(t.stride(-1) == 1 or t.shape[-1] <= 1, f"{name} must have a time stride of 1, got strides {t.stride()}")
+    _require(False, f"{name} must {strides}, got strides {t.stride()}")
+
+
+def _sequence(name, t, shape, dtype, dev):
+    """A (B, D, L) input, or one like it: any strides but the last axis', which is 1."""
+    if t.dtype != dtype or t.shape != shape or t.device != dev or (t.stride(-1) != 1 and shape[-1] > 1):
+        _wrong(name, t, shape, (dtype,), dev, "have a time stride of 1")
 
 
 def _dense(name, t, shape, dtype, dev):
-    _on_gpu(name, t, dev)
-    _require(t.dtype == dtype, f"{name} has dtype {t.dtype}, expected {dtype}")
-    _require(t.shape == shape, f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    _require(t.is_contiguous(), f"{name} must be contiguous")
+    if t.dtype != dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
+        _wrong(name, t, shape, (dtype,), dev, "be contiguous")
 
 
-def _parameter(name, t, shape, like, narrow):
+def _parameter(name, t, shape, dtype, dev, narrow):
     """A parameter in float32 or in the inputs' type; `narrow` is the flag for the latter."""
-    _on_gpu(name, t, like.device)
-    _require(t.dtype == torch.float32 or t.dtype == like.dtype,
-             f"{name} has dtype {t.dtype}, expected torch.float32 or {like.dtype}")
-    _require(t.shape == shape, f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    _require(t.is_contiguous(), f"{name} must be contiguous")
-    return 0 if t.dtype == torch.float32 else narrow
+    own = t.dtype
+    if (own != torch.float32 and own != dtype) or t.shape != shape or t.device != dev or not t.is_contiguous():
+        _wrong(name, t, shape, (torch.float32, dtype), dev, "be contiguous")
+    return 0 if own == torch.float32 else narrow
 
 
-def _lengths(lengths, B, dev):
-    if lengths is not None:
-        _dense("lengths", lengths, (B,), torch.int32, dev)
+def _type_of(t):
+    code = _DTYPES.get(t.dtype)
+    return _dtype_code(t) if code is None else code
 
 
 def _slots(slots, B, dev):
     """The flag for the slots' type."""
     if slots is None:
         return 0
-    _on_gpu("slots", slots, dev)
-    _require(slots.dtype in (torch.int32, torch.int64), f"slots has dtype {slots.dtype}, expected int32 or int64")
-    _require(slots.shape == (B,) and slots.is_contiguous(), f"slots must be a dense {(B,)}, got {tuple(slots.shape)}")
-    return _lib.SELECTIVE_SLOTS_64 if slots.dtype == torch.int64 else 0
+    wide = slots.dtype == torch.int64
+    if (not wide and slots.dtype != torch.int32) or slots.shape != (B,) or slots.device != dev or not slots.is_contiguous():
+        _wrong("slots", slots, (B,), (torch.int32, torch.int64), dev, "be contiguous")
+    return _lib.SELECTIVE_SLOTS_64 if wide else 0
 
 
-def _pool(state, state_out, slots, B, each, dtype, dev):
-    """State pool of a single-token call: (S, *each), and where the new states go."""
-    _on_gpu("state", state, dev)
-    _require(state.dtype == dtype, f"state has dtype {state.dtype}, expected {dtype}")
-    _require(state.dim() == 3 and state.shape[1:] == each, f"state must be (S, {each[0]}, {each[1]}), got {tuple(state.shape)}")
-    _require(state.is_contiguous(), "state must be contiguous")
-    _require(slots is not None or state.shape[0] == B, f"without slots the state must hold {B} rows, got {state.shape[0]}")
+def _pool(state, state_out, slots, B, D, each, dtype, dev):
+    """State pool of a single-token call, (S, D, each), and where the new states go."""
+    _require(state.dim() == 3, "state must be (S, channels, values)")
+    S = state.shape[0]
+    _dense("state", state, (S, D, each), dtype, dev)
+    if slots is None and S != B:
+        _require(False, f"without slots the state must hold {B} rows, got {S}")
     if state_out is None:
         return state
-    _dense("state_out", state_out, state.shape, dtype, dev)
+    _dense("state_out", state_out, (S, D, each), dtype, dev)
     return state_out
 
 
+def _call(dev, entry, *args):
+    """An entry point of the library on `dev` and its current stream."""
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc)
+
+
+def _tracked(*tensors):
+    """Whether autograd follows a call with these arguments."""
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
 def _conv_check(inputs, weight, bias, initial_state, lengths, silu):
-    _require(inputs.dim() == 3 and weight.dim() == 2, "inputs must be (B, D, L) and weight (D, W)")
-    B, D, L = inputs.shape
+    _gpu("inputs", inputs)
+    if inputs.dim() != 3 or weight.dim() != 2:
+        _require(False, "inputs must be (B, D, L) and weight (D, W)")
+    shape, dtype, dev = inputs.shape, inputs.dtype, inputs.device
+    B, D, L = shape
     W = weight.shape[1]
-    _require(2 <= W <= 4, f"weight must have 2, 3 or 4 taps, got {W}")
-    _sequence("inputs", inputs, inputs.shape, inputs)
-    code = _dtype_code(inputs)
-    flags = (_lib.SELECTIVE_SILU if silu else 0) | _parameter("weight", weight, (D, W), inputs, _lib.SELECTIVE_NARROW_WEIGHT)
+    if not 2 <= W <= 4:
+        _require(False, f"weight must have 2, 3 or 4 taps, got {W}")
+    _sequence("inputs", inputs, shape, dtype, dev)
+    code = _type_of(inputs)
+    flags = _parameter("weight", weight, (D, W), dtype, dev, _lib.SELECTIVE_NARROW_WEIGHT)
+    if silu:
+        flags |= _lib.SELECTIVE_SILU
     if bias is not None:
-        flags |= _parameter("bias", bias, (D,), inputs, _lib.SELECTIVE_NARROW_BIAS)
+        flags |= _parameter("bias", bias, (D,), dtype, dev, _lib.SELECTIVE_NARROW_BIAS)
     if initial_state is not None:
-        _dense("initial_state", initial_state, (B, D, W - 1), inputs.dtype, inputs.device)
-    _lengths(lengths, B, inputs.device)
+        _dense("initial_state", initial_state, (B, D, W - 1), dtype, dev)
+    if lengths is not None:
+        _dense("lengths", lengths, (B,), torch.int32, dev)
     return B, D, L, W, code, flags
 
 
@@ -106,10 +138,8 @@ def _conv_forward(inputs, weight, bias, initial_state, lengths, silu, return_sta
     if not out.numel():
         return out, _carried(initial_state, (B, D, W - 1), inputs, inputs.dtype) if return_state else None
     final = torch.empty((B, D, W - 1), dtype=inputs.dtype, device=inputs.device) if return_state else None
-    with _on_device(inputs.device):
-        _lib.check(_raw.fmselective_conv_forward(
-            inputs.data_ptr(), inputs.stride(0), inputs.stride(1), weight.data_ptr(), _ptr(bias), _ptr(initial_state),
-            _ptr(lengths), out.data_ptr(), _ptr(final), B, D, L, W, code, flags, _stream(inputs.device)))
+    _call(inputs.device, _raw.fmselective_conv_forward, inputs.data_ptr(), inputs.stride(0), inputs.stride(1), weight.data_ptr(),
+          _ptr(bias), _ptr(initial_state), _ptr(lengths), out.data_ptr(), _ptr(final), B, D, L, W, code, flags)
     return out, final
 
 
@@ -120,7 +150,7 @@ def _conv_backward(inputs, weight, bias, initial_state, lengths, silu, out_grad,
         out_grad = torch.zeros((B, D, L), dtype=inputs.dtype, device=dev)
     elif out_grad.stride(-1) != 1:
         out_grad = out_grad.contiguous()
-    _sequence("the output's gradient", out_grad, (B, D, L), inputs)
+    _sequence("the output's gradient", out_grad, (B, D, L), inputs.dtype, dev)
     if final_grad is not None:
         final_grad = final_grad.contiguous()
         _dense("the final state's gradient", final_grad, (B, D, W - 1), inputs.dtype, dev)
@@ -135,12 +165,10 @@ def _conv_backward(inputs, weight, bias, initial_state, lengths, silu, out_grad,
     d_state = torch.empty((B, D, W - 1), dtype=inputs.dtype, device=dev) if want_state else None
     need = _raw.fmselective_conv_workspace_bytes(B, D, L, W, code)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _on_device(dev):
-        _lib.check(_raw.fmselective_conv_backward(
-            inputs.data_ptr(), inputs.stride(0), inputs.stride(1), out_grad.data_ptr(), out_grad.stride(0),
-            out_grad.stride(1), weight.data_ptr(), _ptr(bias), _ptr(initial_state), _ptr(final_grad), _ptr(lengths),
-            d_inputs.data_ptr(), d_weight.data_ptr(), _ptr(d_bias), _ptr(d_state), B, D, L, W, code, flags,
-            workspace.data_ptr(), need, _stream(dev)))
+    _call(dev, _raw.fmselective_conv_backward, inputs.data_ptr(), inputs.stride(0), inputs.stride(1), out_grad.data_ptr(),
+          out_grad.stride(0), out_grad.stride(1), weight.data_ptr(), _ptr(bias), _ptr(initial_state), _ptr(final_grad),
+          _ptr(lengths), d_inputs.data_ptr(), d_weight.data_ptr(), _ptr(d_bias), _ptr(d_state), B, D, L, W, code, flags,
+          workspace.data_ptr(), need)
     return d_inputs, d_weight, d_bias, d_state
 
 
@@ -184,7 +212,10 @@ def fm_conv(inputs, weight, bias=None, initial_state=None, lengths=None, silu=Tr
 
     Returns (B, D, L), or that and the final state (B, D, W - 1). Differentiable once, in everything but lengths.
     """
-    out, final = FM_Conv.apply(inputs, weight, bias, initial_state, lengths, silu, return_state)
+    if _tracked(inputs, weight, bias, initial_state):
+        out, final = FM_Conv.apply(inputs, weight, bias, initial_state, lengths, silu, return_state)
+    else:
+        out, final = _conv_forward(inputs, weight, bias, initial_state, lengths, silu, return_state)
     return (out, final) if return_state else out
 
 
@@ -201,107 +232,128 @@ def fm_conv_step(inputs, state, weight, bias=None, slots=None, silu=True, state_
 
     Returns (B, D).
     """
-    _require(inputs.dim() == 2 and weight.dim() == 2, "inputs must be (B, D) and weight (D, W)")
-    B, D = inputs.shape
+    _gpu("inputs", inputs)
+    if inputs.dim() != 2 or weight.dim() != 2:
+        _require(False, "inputs must be (B, D) and weight (D, W)")
+    shape, dtype, dev = inputs.shape, inputs.dtype, inputs.device
+    B, D = shape
     W = weight.shape[1]
-    dev = inputs.device
-    _require(2 <= W <= 4, f"weight must have 2, 3 or 4 taps, got {W}")
-    _sequence("inputs", inputs, inputs.shape, inputs)
-    code = _dtype_code(inputs)
-    flags = (_lib.SELECTIVE_SILU if silu else 0) | _parameter("weight", weight, (D, W), inputs, _lib.SELECTIVE_NARROW_WEIGHT)
+    if not 2 <= W <= 4:
+        _require(False, f"weight must have 2, 3 or 4 taps, got {W}")
+    _sequence("inputs", inputs, shape, dtype, dev)
+    code = _type_of(inputs)
+    flags = _parameter("weight", weight, (D, W), dtype, dev, _lib.SELECTIVE_NARROW_WEIGHT) | _slots(slots, B, dev)
+    if silu:
+        flags |= _lib.SELECTIVE_SILU
     if bias is not None:
-        flags |= _parameter("bias", bias, (D,), inputs, _lib.SELECTIVE_NARROW_BIAS)
-    new = _pool(state, state_out, slots, B, (D, W - 1), inputs.dtype, dev)
-    flags |= _slots(slots, B, dev)
-    if slots is not None and state.shape[0] == 0:
-        return torch.zeros((B, D), dtype=inputs.dtype, device=dev)
-    out = torch.empty((B, D), dtype=inputs.dtype, device=dev)
-    if out.numel():
-        with _on_device(dev):
-            _lib.check(_raw.fmselective_conv_step(
-                inputs.data_ptr(), inputs.stride(0), state.data_ptr(), new.data_ptr(), weight.data_ptr(), _ptr(bias),
-                _ptr(slots), out.data_ptr(), B, D, W, state.shape[0], code, flags, _stream(dev)))
+        flags |= _parameter("bias", bias, (D,), dtype, dev, _lib.SELECTIVE_NARROW_BIAS)
+    new = _pool(state, state_out, slots, B, D, W - 1, dtype, dev)
+    S = state.shape[0]
+    if slots is not None and S == 0:
+        return torch.zeros((B, D), dtype=dtype, device=dev)
+    out = torch.empty(shape, dtype=dtype, device=dev)
+    if B and D:
+        _call(dev, _raw.fmselective_conv_step, inputs.data_ptr(), inputs.stride(0), state.data_ptr(), new.data_ptr(),
+              weight.data_ptr(), _ptr(bias), _ptr(slots), out.data_ptr(), B, D, W, S, code, flags)
     return out
 
 
-def _scan_inputs(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus):
-    """The checked arguments of a call on sequences, as the library takes them."""
-    _require(tokens.dim() == 3 and A.dim() == 2 and write.dim() == 4, "tokens must be (B, D, L), A (D, N), write (B, G, N, L)")
-    B, D, L = tokens.shape
-    N, G = A.shape[1], write.shape[1]
-    dev = tokens.device
-    _sequence("tokens", tokens, tokens.shape, tokens)
-    code = _dtype_code(tokens)
-    _sequence("delta", delta, tokens.shape, tokens)
-    _require(1 <= N <= _lib.SELECTIVE_MAX_STATES, f"A must have 1 to {_lib.SELECTIVE_MAX_STATES} states, got {N}")
+def _channels(tokens, delta, A, skip, gate, delta_bias, G, softplus):
+    """What calls on sequences and for one token check alike: (N, dtype code, flags)."""
+    shape, dtype, dev = tokens.shape, tokens.dtype, tokens.device
+    D, N = shape[1], A.shape[1]
+    _sequence("tokens", tokens, shape, dtype, dev)
+    code = _type_of(tokens)
+    _sequence("delta", delta, shape, dtype, dev)
+    if not 1 <= N <= _lib.SELECTIVE_MAX_STATES:
+        _require(False, f"A must have 1 to {_lib.SELECTIVE_MAX_STATES} states, got {N}")
     _dense("A", A, (D, N), torch.float32, dev)
-    _require(G >= 1 and D % G == 0, f"the groups of write must divide the {D} channels, got {G}")
-    _sequence("write", write, (B, G, N, L), tokens)
-    _sequence("read", read, (B, G, N, L), tokens)
+    if G < 1 or D % G:
+        _require(False, f"the groups of write must divide the {D} channels, got {G}")
     flags = _lib.SELECTIVE_SOFTPLUS if softplus else 0
     if skip is not None:
-        flags |= _parameter("skip", skip, (D,), tokens, _lib.SELECTIVE_NARROW_SKIP)
+        flags |= _parameter("skip", skip, (D,), dtype, dev, _lib.SELECTIVE_NARROW_SKIP)
     if delta_bias is not None:
-        flags |= _parameter("delta_bias", delta_bias, (D,), tokens, _lib.SELECTIVE_NARROW_BIAS)
+        flags |= _parameter("delta_bias", delta_bias, (D,), dtype, dev, _lib.SELECTIVE_NARROW_BIAS)
     if gate is not None:
-        _sequence("gate", gate, tokens.shape, tokens)
+        _sequence("gate", gate, shape, dtype, dev)
+    return N, code, flags
+
+
+def _scan_inputs(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus):
+    """The checked arguments of a call on sequences, as the library takes them, and (B, D, L, N, G, dtype code)."""
+    _gpu("tokens", tokens)
+    if tokens.dim() != 3 or A.dim() != 2 or write.dim() != 4:
+        _require(False, "tokens must be (B, D, L), A (D, N), write (B, G, N, L)")
+    B, D, L = tokens.shape
+    G, dtype, dev = write.shape[1], tokens.dtype, tokens.device
+    N, code, flags = _channels(tokens, delta, A, skip, gate, delta_bias, G, softplus)
+    _sequence("write", write, (B, G, N, L), dtype, dev)
+    _sequence("read", read, (B, G, N, L), dtype, dev)
     if initial_state is not None:
         _dense("initial_state", initial_state, (B, D, N), torch.float32, dev)
-    _lengths(lengths, B, dev)
-    return _lib.ScanInputs(
-        tokens.data_ptr(), delta.data_ptr(), _ptr(gate), write.data_ptr(), read.data_ptr(), _ptr(skip), _ptr(delta_bias),
-        A.data_ptr(), _ptr(initial_state), _ptr(lengths), tokens.stride()[:2], delta.stride()[:2],
-        (0, 0) if gate is None else gate.stride()[:2], write.stride()[:3], read.stride()[:3], B, D, L, N, G, code, flags)
+    if lengths is not None:
+        _dense("lengths", lengths, (B,), torch.int32, dev)
+    z_b, z_d = (0, 0) if gate is None else gate.stride()[:2]
+    packed = _lib.SCAN_INPUTS.pack(
+        tokens.data_ptr(), delta.data_ptr(), _at(gate), write.data_ptr(), read.data_ptr(), _at(skip), _at(delta_bias),
+        A.data_ptr(), _at(initial_state), _at(lengths), *tokens.stride()[:2], *delta.stride()[:2], z_b, z_d,
+        *write.stride()[:3], *read.stride()[:3], B, D, L, N, G, code, flags)
+    return packed, (B, D, L, N, G, code)
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _scan_forward(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus, return_state, save):
     """(out, final state or None, the states that backward starts from or None)"""
-    p = _scan_inputs(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus)
+    packed, sizes = _scan_inputs(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus)
+    B, D, L, N, G, code = sizes
     dev = tokens.device
-    out = torch.empty((p.B, p.D, p.L), dtype=tokens.dtype, device=dev)
-    if not out.numel():
-        return out, _carried(initial_state, (p.B, p.D, p.N), tokens, torch.float32) if return_state else None, None
-    final = torch.empty((p.B, p.D, p.N), dtype=torch.float32, device=dev) if return_state else None
+    out = torch.empty((B, D, L), dtype=tokens.dtype, device=dev)
+    if not (B and D and L):
+        return out, _carried(initial_state, (B, D, N), tokens, torch.float32) if return_state else None, None
+    final = torch.empty((B, D, N), dtype=torch.float32, device=dev) if return_state else None
     marks = None
     if save:
-        marks = torch.empty((p.B, p.D, -(-p.L // _lib.SELECTIVE_MARK), p.N), dtype=torch.float32, device=dev)
-    with _on_device(dev):
-        _lib.check(_raw.fmselective_scan_forward(ctypes.addressof(p), out.data_ptr(), _ptr(final), _ptr(marks), _stream(dev)))
+        marks = torch.empty((B, D, -(-L // _lib.SELECTIVE_MARK), N), dtype=torch.float32, device=dev)
+    need = _raw.fmselective_scan_workspace_bytes(*sizes, 0)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(dev, _raw.fmselective_scan_forward, packed, out.data_ptr(), _ptr(final), _ptr(marks), _ptr(workspace), need)
     return out, final, marks
 
 
 def _scan_backward(inputs, softplus, marks, out_grad, final_grad, want_state):
     """Gradients in the order of the inputs, None for absent ones."""
     tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths = inputs
-    p = _scan_inputs(*inputs, softplus)
+    packed, sizes = _scan_inputs(*inputs, softplus)
+    B, D, L, N, G, code = sizes
     dev, dtype = tokens.device, tokens.dtype
-    shape = (p.B, p.D, p.L)
     if out_grad is None:
-        out_grad = torch.zeros(shape, dtype=dtype, device=dev)
+        out_grad = torch.zeros((B, D, L), dtype=dtype, device=dev)
     elif out_grad.stride(-1) != 1:
         out_grad = out_grad.contiguous()
-    _sequence("the output's gradient", out_grad, shape, tokens)
+    _sequence("the output's gradient", out_grad, (B, D, L), dtype, dev)
     if final_grad is not None:
         final_grad = final_grad.contiguous()
-        _dense("the final state's gradient", final_grad, (p.B, p.D, p.N), torch.float32, dev)
-    if not tokens.numel():
+        _dense("the final state's gradient", final_grad, (B, D, N), torch.float32, dev)
+    if not (B and D and L):
         d_state = None
         if want_state:
-            d_state = torch.zeros((p.B, p.D, p.N), dtype=torch.float32, device=dev) if final_grad is None else final_grad
+            d_state = torch.zeros((B, D, N), dtype=torch.float32, device=dev) if final_grad is None else final_grad
         zeros = [None if t is None else torch.zeros_like(t) for t in (tokens, delta, A, write, read, skip, gate, delta_bias)]
         return (*zeros, d_state)
     new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
     grads = [new(t) for t in (tokens, delta, A, write, read, skip, gate, delta_bias)]
     d_tokens, d_delta, d_A, d_write, d_read, d_skip, d_gate, d_bias = grads
-    d_state = torch.empty((p.B, p.D, p.N), dtype=torch.float32, device=dev) if want_state else None
-    need = _raw.fmselective_scan_workspace_bytes(p.B, p.D, p.L, p.N, p.G, p.dtype)
+    d_state = torch.empty((B, D, N), dtype=torch.float32, device=dev) if want_state else None
+    need = _raw.fmselective_scan_workspace_bytes(*sizes, 1)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    o = _lib.ScanGrads(out_grad.data_ptr(), out_grad.stride()[:2], _ptr(final_grad), marks.data_ptr(), d_tokens.data_ptr(),
-                       d_delta.data_ptr(), _ptr(d_gate), d_write.data_ptr(), d_read.data_ptr(), d_A.data_ptr(),
-                       _ptr(d_state), _ptr(d_skip), _ptr(d_bias))
-    with _on_device(dev):
-        _lib.check(_raw.fmselective_scan_backward(ctypes.addressof(p), ctypes.addressof(o), workspace.data_ptr(), need,
-                                                  _stream(dev)))
+    o = _lib.SCAN_GRADS.pack(out_grad.data_ptr(), *out_grad.stride()[:2], _at(final_grad), marks.data_ptr(),
+                             d_tokens.data_ptr(), d_delta.data_ptr(), _at(d_gate), d_write.data_ptr(), d_read.data_ptr(),
+                             d_A.data_ptr(), _at(d_state), _at(d_skip), _at(d_bias))
+    _call(dev, _raw.fmselective_scan_backward, packed, o, workspace.data_ptr(), need)
     return (*grads, d_state)
 
 
@@ -356,8 +408,11 @@ def fm_selective_scan(tokens, delta, A, write, read, skip=None, gate=None, delta
     """
     if write.dim() == 3 and read.dim() == 3:
         write, read = write.unsqueeze(1), read.unsqueeze(1)
-    out, final = FM_Selective.apply(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus,
-                                    return_state)
+    inputs = (tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths)
+    if _tracked(*inputs):
+        out, final = FM_Selective.apply(*inputs, softplus, return_state)
+    else:
+        out, final, _ = _scan_forward(*inputs, softplus, return_state, False)
     return (out, final) if return_state else out
 
 
@@ -378,36 +433,25 @@ def fm_selective_step(tokens, state, delta, A, write, read, skip=None, gate=None
     """
     if write.dim() == 2 and read.dim() == 2:
         write, read = write.unsqueeze(1), read.unsqueeze(1)
-    _require(tokens.dim() == 2 and A.dim() == 2 and write.dim() == 3, "tokens must be (B, D), A (D, N), write (B, G, N)")
-    B, D = tokens.shape
-    N, G = A.shape[1], write.shape[1]
-    dev = tokens.device
-    _sequence("tokens", tokens, tokens.shape, tokens)
-    code = _dtype_code(tokens)
-    _sequence("delta", delta, tokens.shape, tokens)
-    _require(1 <= N <= _lib.SELECTIVE_MAX_STATES, f"A must have 1 to {_lib.SELECTIVE_MAX_STATES} states, got {N}")
-    _dense("A", A, (D, N), torch.float32, dev)
-    _require(G >= 1 and D % G == 0, f"the groups of write must divide the {D} channels, got {G}")
-    _sequence("write", write, (B, G, N), tokens)
-    _sequence("read", read, (B, G, N), tokens)
-    flags = (_lib.SELECTIVE_SOFTPLUS if softplus else 0) | _slots(slots, B, dev)
-    if skip is not None:
-        flags |= _parameter("skip", skip, (D,), tokens, _lib.SELECTIVE_NARROW_SKIP)
-    if delta_bias is not None:
-        flags |= _parameter("delta_bias", delta_bias, (D,), tokens, _lib.SELECTIVE_NARROW_BIAS)
-    if gate is not None:
-        _sequence("gate", gate, tokens.shape, tokens)
-    new = _pool(state, state_out, slots, B, (D, N), torch.float32, dev)
-    if slots is not None and state.shape[0] == 0:
-        return torch.zeros((B, D), dtype=tokens.dtype, device=dev)
-    out = torch.empty((B, D), dtype=tokens.dtype, device=dev)
-    if out.numel():
-        p = _lib.ScanInputs(
-            tokens.data_ptr(), delta.data_ptr(), _ptr(gate), write.data_ptr(), read.data_ptr(), _ptr(skip),
-            _ptr(delta_bias), A.data_ptr(), state.data_ptr(), None, (tokens.stride(0), 0), (delta.stride(0), 0),
-            (0 if gate is None else gate.stride(0), 0), (write.stride(0), write.stride(1), 0),
-            (read.stride(0), read.stride(1), 0), B, D, 1, N, G, code, flags)
-        with _on_device(dev):
-            _lib.check(_raw.fmselective_scan_step(ctypes.addressof(p), new.data_ptr(), _ptr(slots), state.shape[0],
-                                                  out.data_ptr(), _stream(dev)))
+    _gpu("tokens", tokens)
+    if tokens.dim() != 2 or A.dim() != 2 or write.dim() != 3:
+        _require(False, "tokens must be (B, D), A (D, N), write (B, G, N)")
+    shape, dtype, dev = tokens.shape, tokens.dtype, tokens.device
+    B, D = shape
+    G = write.shape[1]
+    N, code, flags = _channels(tokens, delta, A, skip, gate, delta_bias, G, softplus)
+    _sequence("write", write, (B, G, N), dtype, dev)
+    _sequence("read", read, (B, G, N), dtype, dev)
+    flags |= _slots(slots, B, dev)
+    new = _pool(state, state_out, slots, B, D, N, torch.float32, dev)
+    S = state.shape[0]
+    if slots is not None and S == 0:
+        return torch.zeros(shape, dtype=dtype, device=dev)
+    out = torch.empty(shape, dtype=dtype, device=dev)
+    if B and D:
+        packed = _lib.SCAN_INPUTS.pack(
+            tokens.data_ptr(), delta.data_ptr(), _at(gate), write.data_ptr(), read.data_ptr(), _at(skip), _at(delta_bias),
+            A.data_ptr(), state.data_ptr(), 0, tokens.stride(0), 0, delta.stride(0), 0, 0 if gate is None else gate.stride(0), 0,
+            *write.stride(), *read.stride(), B, D, 1, N, G, code, flags)
+        _call(dev, _raw.fmselective_scan_step, packed, new.data_ptr(), _ptr(slots), S, out.data_ptr())
     return out

@@ -89,10 +89,17 @@ typedef struct fmselective_scan_inputs {
     uint32_t flags;
 } fmselective_scan_inputs;
 
+/* Rows that are too few to fill the GPU are cut along time; what passes between the pieces goes through a workspace.
+ * The forward call takes NULL (rows are then scanned in one piece, the same results up to rounding), the backward
+ * call needs its own, which holds its partial sums too. Bytes that a call of these sizes can use; 0 where none or
+ * where the sizes are not valid. */
+size_t fmselective_scan_workspace_bytes(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int dtype, int backward);
+
 /* out (B, D, L); final_state (B, D, N) or NULL; marks (B, D, ceil(L / FMSELECTIVE_MARK), N) float32 or NULL: the
  * states before every FMSELECTIVE_MARK steps, which the backward call needs (those at or beyond a row's length
  * are not written). */
-int fmselective_scan_forward(const fmselective_scan_inputs* in, void* out, float* final_state, float* marks, void* stream);
+int fmselective_scan_forward(const fmselective_scan_inputs* in, void* out, float* final_state, float* marks, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 typedef struct fmselective_scan_grads {
     const void* out_grad;           /* (B, D, L), strided */
@@ -105,8 +112,6 @@ typedef struct fmselective_scan_grads {
     void *skip, *delta_bias;        /* (D), of the parameters' types, NULL where the inputs' are */
 } fmselective_scan_grads;
 
-/* Bytes of workspace that the backward call needs (partial sums over channels and batch); 0 where sizes are not valid. */
-size_t fmselective_scan_workspace_bytes(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int dtype);
 int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselective_scan_grads* grads, void* workspace,
                               size_t workspace_bytes, void* stream);
 

@@ -185,7 +185,8 @@ def test_conv_steps_are_the_sequence(m):
 
 SCAN_SHAPES = [  # B, D, L, N, G
     (1, 1, 1, 1, 1), (2, 3, 2, 2, 1), (1, 4, 7, 3, 2), (2, 6, 9, 16, 3), (3, 17, 40, 5, 1), (1, 8, 127, 16, 2),
-    (1, 33, 128, 8, 1), (2, 20, 129, 17, 1), (1, 5, 300, 33, 1), (2, 4, 513, 4, 4), (1, 2, 1100, 16, 1), (70, 2, 3, 4, 1)]
+    (1, 33, 128, 8, 1), (2, 20, 129, 17, 1), (1, 5, 300, 33, 1), (2, 4, 513, 4, 4), (1, 2, 1100, 16, 1), (70, 2, 3, 4, 1),
+    (1, 2, 2700, 3, 1), (2, 3, 5000, 2, 1), (260, 40, 140, 3, 1)]  # rows cut along time; two sets of channels a lane
 
 
 def scan_case(shape, dtype, variant, seed=0):

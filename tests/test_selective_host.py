@@ -74,13 +74,9 @@ def on_cpu(monkeypatch, modules):
         def __getattr__(self, name):
             raise AssertionError(f"{name} was called before the arguments were checked")
 
-    def same_device(name, t, dev):
-        if t.device != dev:
-            raise RuntimeError(f"{name} is on {t.device}, expected {dev}")
-
     for mod in modules:
         monkeypatch.setattr(mod, "_raw", NoLaunch())
-        monkeypatch.setattr(mod, "_on_gpu", same_device)
+        monkeypatch.setattr(mod, "_gpu", lambda name, t: None)
 
 
 def refuses(call, good, changes):
@@ -135,22 +131,25 @@ def test_conv_checks_its_arguments(monkeypatch):
 
 
 def scan_inputs(_lib, **change):
-    a = dict(tokens=P, delta=2 * P, gate=None, write=3 * P, read=4 * P, skip=None, delta_bias=None, A=5 * P, initial_state=None,
-             lengths=None, tokens_strides=(24, 8), delta_strides=(24, 8), gate_strides=(24, 8), write_strides=(32, 32, 8),
+    a = dict(tokens=P, delta=2 * P, gate=0, write=3 * P, read=4 * P, skip=0, delta_bias=0, A=5 * P, initial_state=0, lengths=0,
+             tokens_strides=(24, 8), delta_strides=(24, 8), gate_strides=(24, 8), write_strides=(32, 32, 8),
              read_strides=(32, 32, 8), B=2, D=3, L=8, N=4, G=1, dtype=2, flags=0)
-    return _lib.ScanInputs(**{**a, **change})
+    return packed(_lib.SCAN_INPUTS, {**a, **{k: v or 0 for k, v in change.items()}}, len(a))
+
+
+def packed(form, fields, count):
+    assert len(fields) == count  # no field by a wrong name
+    return form.pack(*[x for v in fields.values() for x in (v if isinstance(v, tuple) else (v,))])
 
 
 def test_scan_rejects(lib):
-    import ctypes
-
     from fm_amd import _lib
 
-    def fwd(out=7 * P, final=None, marks=None, **change):
+    def fwd(out=7 * P, final=None, marks=None, ws=None, ws_bytes=0, **change):
         p = scan_inputs(_lib, **change)
-        return lib.fmselective_scan_forward(ctypes.addressof(p), out, final, marks, None)
+        return lib.fmselective_scan_forward(p, out, final, marks, ws, ws_bytes, None)
 
-    assert lib.fmselective_scan_forward(None, P, None, None, None) == code("NULL")
+    assert lib.fmselective_scan_forward(None, P, None, None, None, 0, None) == code("NULL")
     assert fwd(out=None) == code("NULL") and fwd(tokens=None) == code("NULL") and fwd(read=None) == code("NULL")
     assert fwd(N=0) == code("SHAPE") and fwd(N=257) == code("SHAPE") and fwd(G=2) == code("SHAPE") and fwd(L=0) == code("SHAPE")
     assert fwd(write_strides=(32, 32, -8)) == code("SHAPE") and fwd(B=1 << 30, D=4) == code("SHAPE")
@@ -158,13 +157,16 @@ def test_scan_rejects(lib):
     assert fwd(out=P + 32) == code("ALIAS") and fwd(final=5 * P) == code("ALIAS") and fwd(marks=7 * P) == code("ALIAS")
     assert fwd(initial_state=6 * P, final=6 * P) == code("ALIAS")
     need = lib.fmselective_scan_workspace_bytes
-    assert need(2, 3, 8, 4, 1, 2) > 0 and need(2, 3, 8, 4, 2, 2) == 0 and need(2, 3, 0, 4, 1, 2) == 0
+    assert need(2, 3, 8, 4, 1, 2, 1) > 0 and need(2, 3, 8, 4, 2, 2, 1) == 0 and need(2, 3, 0, 4, 1, 2, 1) == 0
+    assert need(2, 3, 8, 4, 1, 2, 0) == 0 and need(1, 3, 1 << 16, 4, 1, 2, 0) > 0 and need(8, 4096, 1 << 16, 4, 1, 2, 0) == 0
+    long = dict(L=1 << 16, tokens_strides=(3 << 16, 1 << 16), delta_strides=(3 << 16, 1 << 16))
+    assert fwd(ws=P, ws_bytes=1 << 30, **long) == code("ALIAS") and fwd(ws=7 * P + 64, ws_bytes=1 << 30, **long) == code("ALIAS")
 
     def bwd(ws=20 * P, ws_bytes=1 << 30, inputs={}, **change):
-        g = dict(out_grad=7 * P, out_grad_strides=(24, 8), final_state_grad=None, marks=8 * P, tokens=9 * P, delta=10 * P,
-                 gate=None, write=11 * P, read=12 * P, A=13 * P, initial_state=None, skip=None, delta_bias=None)
-        p, o = scan_inputs(_lib, **inputs), _lib.ScanGrads(**{**g, **change})
-        return lib.fmselective_scan_backward(ctypes.addressof(p), ctypes.addressof(o), ws, ws_bytes, None)
+        g = dict(out_grad=7 * P, out_grad_strides=(24, 8), final_state_grad=0, marks=8 * P, tokens=9 * P, delta=10 * P, gate=0,
+                 write=11 * P, read=12 * P, A=13 * P, initial_state=0, skip=0, delta_bias=0)
+        o = packed(_lib.SCAN_GRADS, {**g, **{k: v or 0 for k, v in change.items()}}, len(g))
+        return lib.fmselective_scan_backward(scan_inputs(_lib, **inputs), o, ws, ws_bytes, None)
 
     assert bwd(marks=None) == code("NULL") and bwd(write=None) == code("NULL")
     assert bwd(gate=14 * P) == code("NULL") and bwd(inputs=dict(skip=15 * P)) == code("NULL")
@@ -173,7 +175,7 @@ def test_scan_rejects(lib):
 
     def step(state=6 * P, new=6 * P, slots=None, S=2, out=7 * P, **change):
         p = scan_inputs(_lib, initial_state=state, **change)
-        return lib.fmselective_scan_step(ctypes.addressof(p), new, slots, S, out, None)
+        return lib.fmselective_scan_step(p, new, slots, S, out, None)
 
     assert step(state=None) == code("NULL") and step(out=None) == code("NULL")
     assert step(S=3) == code("SHAPE") and step(S=0, slots=16 * P) == code("SHAPE") and step(new=6 * P + 16) == code("ALIAS")
