@@ -46,31 +46,50 @@ __device__ __forceinline__ void conv_taps(const void* weight, const void* bias, 
 struct ConvRows {
     int64_t batch_stride, channel_stride, L;
     int32_t rows, D;
-    uint32_t tiles;         // blocks a row takes (1 where a block takes whole rows)
-    uint32_t rows_per_block;
-    uint32_t chunks;        // of a row
-    uint32_t magic;         // ceil(2^16 / chunks), for rows_per_block > 1
+    uint32_t units;           // of 64 * CH chunks a row has, a wave each (long rows)
+    uint32_t rows_per_block;  // (short rows)
+    uint32_t chunks;          // of a row
+    uint32_t magic;           // ceil(2^16 / chunks) (short rows)
 };
 
-// One chunk of 16 bytes a thread; the W - 1 values before it are a second, 8-byte load that the L1 answers.
-// Short rows are packed: a block takes as many whole rows as it has threads for.
+// A chunk's outputs from its inputs and the W - 1 values before it
 template <typename T, int W>
-__global__ __launch_bounds__(256) void conv_forward_kernel(const T* __restrict__ inputs, const void* __restrict__ weight,
-                                                           const void* __restrict__ bias, const T* __restrict__ initial,
-                                                           const int32_t* __restrict__ lengths, T* __restrict__ out,
-                                                           T* __restrict__ final_state, ConvRows g, unsigned flags) {
-    constexpr int E = Elem<T>::E;
-    uint32_t row, chunk;
-    if (g.rows_per_block > 1) {
-        const uint32_t r = (threadIdx.x * g.magic) >> 16;
-        if (r >= g.rows_per_block) return;
-        row = blockIdx.x * g.rows_per_block + r;
-        chunk = threadIdx.x - r * g.chunks;
-    } else {
-        row = g.tiles == 1 ? blockIdx.x : blockIdx.x / g.tiles;
-        chunk = (blockIdx.x - row * g.tiles) * blockDim.x + threadIdx.x;
+__device__ __forceinline__ void conv_chunk(const float (&f)[Elem<T>::E], const float (&before)[W - 1], const float (&w)[W], float bias,
+                                           bool silu, float (&y)[Elem<T>::E]) {
+    auto at = [&](int i) { return i < 0 ? before[i + W - 1] : f[i]; };
+#pragma unroll
+    for (int k = 0; k < Elem<T>::E; ++k) {
+        float v = bias;
+#pragma unroll
+        for (int j = 0; j < W; ++j) v = __builtin_fmaf(w[j], at(k - (W - 1) + j), v);
+        y[k] = v;
     }
-    if (row >= (uint32_t)g.rows || chunk >= g.chunks) return;
+    if (silu) {
+#pragma unroll
+        for (int k = 0; k < Elem<T>::E; ++k) y[k] *= sigmoid(y[k]);
+    }
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void conv_final_state(const T* __restrict__ x, const T* __restrict__ state, int64_t len, T* __restrict__ to) {
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) {
+        const int64_t p = len - (W - 1) + i;
+        to[i] = p >= 0 ? x[p] : (state ? state[p + W - 1] : (T)0.0f);
+    }
+}
+
+// Rows of at most 64 chunks of 16 bytes: a chunk a thread, as many whole rows a block as it has threads for. The W - 1
+// values before a chunk are a second, 8-byte load that the L1 answers.
+template <typename T, int W>
+__global__ __launch_bounds__(256) void conv_forward_short_kernel(const T* __restrict__ inputs, const void* __restrict__ weight,
+                                                                 const void* __restrict__ bias, const T* __restrict__ initial,
+                                                                 const int32_t* __restrict__ lengths, T* __restrict__ out,
+                                                                 T* __restrict__ final_state, ConvRows g, unsigned flags) {
+    constexpr int E = Elem<T>::E;
+    const uint32_t r = (threadIdx.x * g.magic) >> 16;
+    const uint32_t row = blockIdx.x * g.rows_per_block + r, chunk = threadIdx.x - r * g.chunks;
+    if (r >= g.rows_per_block || row >= (uint32_t)g.rows) return;
     const uint32_t b = row / (uint32_t)g.D, d = row - b * g.D;
     const int64_t len = row_length(lengths, b, g.L), t0 = (int64_t)chunk * E;
     const T* x = inputs + b * g.batch_stride + d * g.channel_stride;
@@ -79,23 +98,62 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(const T* __restrict__
     load_values<T, E>(x, t0, len, f);
     values_before<T, W>(x, t0, len, state, before);
     conv_taps<T, W>(weight, bias, d, flags, w, bv);
-    auto at = [&](int i) { return i < 0 ? before[i + W - 1] : f[i]; };
+    conv_chunk<T, W>(f, before, w, bv, flags & FMSELECTIVE_SILU, y);
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-        float v = bv;
-#pragma unroll
-        for (int j = 0; j < W; ++j) v = __builtin_fmaf(w[j], at(k - (W - 1) + j), v);
-        if (flags & FMSELECTIVE_SILU) v *= sigmoid(v);
-        y[k] = t0 + k < len ? v : 0.0f;
-    }
+    for (int k = 0; k < E; ++k) y[k] = t0 + k < len ? y[k] : 0.0f;
     store_values<T, E>(out + (int64_t)row * g.L, t0, g.L, y);
-    if (final_state && chunk == 0) {
+    if (final_state && chunk == 0) conv_final_state<T, W>(x, state, len, final_state + (int64_t)row * (W - 1));
+}
+
+// Long rows: a wave takes CH * 64 chunks of a row, all its loads in flight at once; a lane's values before its chunk come
+// from the lane below, lane 0's from lane 63 of the chunks before, and from memory once a wave.
+template <typename T, int W, int CH>
+__global__ __launch_bounds__(256) void conv_forward_kernel(const T* __restrict__ inputs, const void* __restrict__ weight,
+                                                           const void* __restrict__ bias, const T* __restrict__ initial,
+                                                           const int32_t* __restrict__ lengths, T* __restrict__ out,
+                                                           T* __restrict__ final_state, ConvRows g, unsigned flags) {
+    constexpr int E = Elem<T>::E;
+    const int lane = threadIdx.x & 63;
+    const uint32_t at = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const uint32_t row = at / g.units, unit = at - row * g.units;
+    if (row >= (uint32_t)g.rows) return;
+    const uint32_t b = row / (uint32_t)g.D, d = row - b * g.D;
+    const int64_t len = row_length(lengths, b, g.L), start = (int64_t)unit * (CH * 64 * E);
+    const T* x = inputs + b * g.batch_stride + d * g.channel_stride;
+    const T* state = initial ? initial + (int64_t)row * (W - 1) : nullptr;
+    T* y_row = out + (int64_t)row * g.L;
+    const bool full = start + CH * 64 * E <= len;
+    u32x4 raw[CH];
+    if (full) {
+#pragma unroll
+        for (int j = 0; j < CH; ++j) raw[j] = fmscan::load16<T, true, false>(x + start + (j * 64 + lane) * E);
+    } else {
+#pragma unroll
+        for (int j = 0; j < CH; ++j) raw[j] = fmscan::load_chunk<T, false, false>(x, start + (j * 64 + lane) * E, len, 0u);
+    }
+    float w[W], bv, first[W - 1];
+    if (lane == 0) values_before<T, W>(x, start, len, state, first);
+    conv_taps<T, W>(weight, bias, d, flags, w, bv);
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+        float f[E], before[W - 1], y[E];
+        Elem<T>::unpack(raw[j], f);
 #pragma unroll
         for (int i = 0; i < W - 1; ++i) {
-            const int64_t p = len - (W - 1) + i;
-            final_state[(int64_t)row * (W - 1) + i] = p >= 0 ? x[p] : (state ? state[p + W - 1] : (T)0.0f);
+            before[i] = fmscan::dpp<fmscan::kWaveShr1>(first[i], f[E - (W - 1) + i]);  // lane 0 keeps `first`
+            first[i] = fmscan::lane63(f[E - (W - 1) + i]);
+        }
+        conv_chunk<T, W>(f, before, w, bv, flags & FMSELECTIVE_SILU, y);
+        const int64_t t0 = start + (j * 64 + lane) * E;
+        if (full) {
+            fmscan::store16<T, false>(y_row + t0, Elem<T>::pack(y));
+        } else {
+#pragma unroll
+            for (int k = 0; k < E; ++k) y[k] = t0 + k < len ? y[k] : 0.0f;
+            store_values<T, E>(y_row, t0, g.L, y);
         }
     }
+    if (final_state && unit == 0 && lane == 0) conv_final_state<T, W>(x, state, len, final_state + (int64_t)row * (W - 1));
 }
 
 struct ConvBack {
@@ -116,6 +174,8 @@ __device__ __forceinline__ float conv_dpre(float pre, float dy, bool silu) {
 // chunk come from the next lane, and the last lane's from the tile before (lane 0's, kept). The gradients of
 // weight and bias are summed over the whole walk in registers and across the lanes once. Rows of fewer than
 // 64 chunks share a wave, 2^lanes_log2 lanes each.
+// Tiles that lie wholly inside the row are loaded four at a time, by loads without a condition; the others come first
+// in the walk.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void conv_backward_kernel(const T* __restrict__ inputs, const T* __restrict__ out_grad,
                                                             const void* __restrict__ weight, const void* __restrict__ bias,
@@ -140,6 +200,7 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(const T* __restrict_
     const T* dy = out_grad + b * g.grad_batch_stride + d * g.grad_channel_stride;
     const T* state = initial ? initial + (int64_t)row * H : nullptr;
     const T* fg = final_grad ? final_grad + (int64_t)row * H : nullptr;
+    T* dx_row = inputs_grad + (int64_t)row * g.L;
     float w[W], bv;
     conv_taps<T, W>(weight, bias, d, flags, w, bv);
 
@@ -166,20 +227,39 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(const T* __restrict_
     float dpre[E + H];
 #pragma unroll
     for (int k = 0; k < E + H; ++k) dpre[k] = 0.0f;
-    for (int32_t i = hi - 1; i >= lo; --i) {
+
+    // `first`: the values before the row's first lane's chunk, in that lane; FULL: every step of the tile counts and none
+    // is in the final state's gradient
+    auto work = [&](auto full_tag, int32_t i, const u32x4& raw_x, const u32x4& raw_dy, const float (&first)[H]) {
+        constexpr bool FULL = decltype(full_tag)::value;
         const int64_t t0 = i * tile + (int64_t)c * E;
         float f[E], gy[E], before[H], dx[E];
-        load_values<T, E>(x, t0, len, f);
-        load_values<T, E>(dy, t0, len, gy);
-        values_before<T, W>(x, t0, len, state, before);
+        Elem<T>::unpack(raw_x, f);
+        Elem<T>::unpack(raw_dy, gy);
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+            const float below = fmscan::dpp<fmscan::kWaveShr1>(0.0f, f[E - H + k]);
+            before[k] = c == 0 ? first[k] : below;
+        }
         auto at = [&](int p) { return p < 0 ? before[p + H] : f[p]; };
+        if (silu) {
+            float pre[E];
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                pre[k] = bv;
+#pragma unroll
+                for (int j = 0; j < W; ++j) pre[k] = __builtin_fmaf(w[j], at(k - H + j), pre[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < E; ++k) dpre[k] = conv_dpre(pre[k], gy[k], true);
+        } else {
+#pragma unroll
+            for (int k = 0; k < E; ++k) dpre[k] = gy[k];
+        }
 #pragma unroll
         for (int k = 0; k < E; ++k) {
-            float pre = bv;
-#pragma unroll
-            for (int j = 0; j < W; ++j) pre = __builtin_fmaf(w[j], at(k - H + j), pre);
-            const bool in = t0 + k < len;
-            dpre[k] = in ? conv_dpre(pre, gy[k], silu) : 0.0f;
+            const bool in = FULL || t0 + k < len;
+            if (!FULL) dpre[k] = in ? dpre[k] : 0.0f;
             // (a position that does not count adds nothing, whatever stands before it)
 #pragma unroll
             for (int j = 0; j < W; ++j) dw[j] = __builtin_fmaf(dpre[k], in ? at(k - H + j) : 0.0f, dw[j]);
@@ -196,12 +276,58 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(const T* __restrict_
             float v = 0.0f;
 #pragma unroll
             for (int j = 0; j < W; ++j) v = __builtin_fmaf(w[j], dpre[k + H - j], v);
-            const int64_t p = t0 + k - (len - H);  // place in the final state
-            if (fg && p >= 0 && p < H && t0 + k < len) v += Elem<T>::widen(fg[p]);
-            dx[k] = t0 + k < len ? v : 0.0f;
+            if (!FULL) {
+                const int64_t p = t0 + k - (len - H);  // place in the final state
+                if (fg && p >= 0 && p < H && t0 + k < len) v += Elem<T>::widen(fg[p]);
+            }
+            dx[k] = FULL || t0 + k < len ? v : 0.0f;
         }
-        store_values<T, E>(inputs_grad + (int64_t)row * g.L, t0, L, dx);
+        if constexpr (FULL) fmscan::store16<T, false>(dx_row + t0, Elem<T>::pack(dx));
+        else store_values<T, E>(dx_row, t0, L, dx);
+    };
+    auto fetch_first = [&](int32_t i, float (&first)[H]) {
+#pragma unroll
+        for (int k = 0; k < H; ++k) first[k] = 0.0f;
+        if (c == 0) values_before<T, W>(x, i * tile, len, state, first);
+    };
+    int32_t i = hi - 1;
+    // the final state's gradient reaches H positions back, so a tile is full only with H more steps behind it;
+    // rows that share a wave have one tile, of their own lengths
+    for (; i >= lo && (g.lanes_log2 < 6 || (i + 1) * tile + (fg ? H : 0) > len); --i) {
+        const int64_t t0 = i * tile + (int64_t)c * E;
+        float first[H];
+        fetch_first(i, first);
+        work(std::false_type{}, i, fmscan::load_chunk<T, false, false>(x, t0, len, 0u),
+             fmscan::load_chunk<T, false, false>(dy, t0, len, 0u), first);
     }
+    auto walk = [&](auto count_tag) {
+        constexpr int CH = decltype(count_tag)::value;
+        u32x4 raw_x[CH], raw_dy[CH];
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+            raw_x[j] = fmscan::load16<T, false, false>(x + (i - j) * tile + lane * E);
+            raw_dy[j] = fmscan::load16<T, true, false>(dy + (i - j) * tile + lane * E);
+        }
+        float first[H];
+        fetch_first(i - (CH - 1), first);
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+            float before[H];
+            if (j + 1 < CH) {  // lane 63 of the tile before, which is here
+                float f[E];
+                Elem<T>::unpack(raw_x[j + 1 < CH ? j + 1 : j], f);
+#pragma unroll
+                for (int k = 0; k < H; ++k) before[k] = fmscan::lane63(f[E - H + k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < H; ++k) before[k] = first[k];
+            }
+            work(std::true_type{}, i - j, raw_x[j], raw_dy[j], before);
+        }
+        i -= CH;
+    };
+    while (i - lo >= 3) walk(std::integral_constant<int, 4>{});
+    while (i >= lo) walk(std::integral_constant<int, 1>{});
     if (initial_grad && live && seg == 0 && c == 0) {
 #pragma unroll
         for (int i = 0; i < H; ++i) {
@@ -214,11 +340,22 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(const T* __restrict_
             initial_grad[(int64_t)row * H + i] = (T)v;
         }
     }
+    const int64_t at = (int64_t)seg * g.rows + row;
+    if (lanes == 64) {  // (live: a wave without a row has none to write)
+#pragma unroll
+        for (int j = 0; j < W; ++j) dw[j] = wave_sum_high(dw[j]);
+        db = wave_sum_high(db);
+        if (live && lane == 63) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) weight_part[at * W + j] = dw[j];
+            bias_part[at] = db;
+        }
+        return;
+    }
     auto over_lanes = [&](float v) {
         for (int s = lanes >> 1; s > 0; s >>= 1) v += __shfl_xor(v, s);
         return v;
     };
-    const int64_t at = (int64_t)seg * g.rows + row;
 #pragma unroll
     for (int j = 0; j < W; ++j) {
         const float v = over_lanes(dw[j]);

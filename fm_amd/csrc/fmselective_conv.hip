@@ -65,21 +65,25 @@ int fmselective_conv_forward(const void* inputs, int64_t batch_stride, int64_t c
     ConvRows g = {batch_stride, channel_stride, L, (int32_t)(B * D), (int32_t)D, 1, 1, 0, 0};
     const int E = 16 / es;
     g.chunks = (uint32_t)((L + E - 1) / E);
-    unsigned threads = 256;
-    if (g.chunks <= 64) {
+    const int each = g.chunks <= 64 ? 1 : g.chunks <= 128 ? 2 : 4;  // chunks a lane
+    int64_t blocks;
+    if (each == 1) {
         g.rows_per_block = 256 / g.chunks;
         g.magic = (65536 + g.chunks - 1) / g.chunks;
+        blocks = ((int64_t)g.rows + g.rows_per_block - 1) / g.rows_per_block;
     } else {
-        g.tiles = (g.chunks + 255) / 256;
-        threads = ((g.chunks + g.tiles - 1) / g.tiles + 63) / 64 * 64;
+        g.units = (g.chunks + 64 * each - 1) / (64 * each);
+        blocks = ((int64_t)g.rows * g.units + 3) / 4;
+        if (blocks > INT32_MAX / 4) return fail(FMSCAN_E_SHAPE, "%s: B * D * L is too large for one launch", who);
     }
-    const int64_t blocks = ((int64_t)g.rows + g.rows_per_block - 1) / g.rows_per_block * g.tiles;
-    if (blocks > INT32_MAX) return fail(FMSCAN_E_SHAPE, "%s: B * D * L is too large for one launch", who);
     with_dtype(dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
         with_taps(W, [&](auto wt) {
-            fmselective::conv_forward_kernel<T, decltype(wt)::value><<<(unsigned)blocks, threads, 0, (hipStream_t)stream>>>(
-                (const T*)inputs, weight, bias, (const T*)initial_state, lengths, (T*)out, (T*)final_state, g, flags);
+            constexpr int TAPS = decltype(wt)::value;
+            const auto kernel = each == 1 ? fmselective::conv_forward_short_kernel<T, TAPS>
+                                : each == 2 ? fmselective::conv_forward_kernel<T, TAPS, 2> : fmselective::conv_forward_kernel<T, TAPS, 4>;
+            kernel<<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>((const T*)inputs, weight, bias, (const T*)initial_state,
+                                                                      lengths, (T*)out, (T*)final_state, g, flags);
         });
     });
     return launched("convolution (forward)");

@@ -66,6 +66,27 @@ __device__ __forceinline__ void store_values(T* __restrict__ row, int64_t t0, in
     }
 }
 
+// Sums by DPP, a lane's source outside its row being zero
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ float dpp_or_zero(float v) {
+    return u2f((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f2u(v), CTRL, ROW_MASK, 0xf, ROW_MASK == 0xf));
+}
+// Lane 15 of each row of 16: the sum over the row
+__device__ __forceinline__ float row_sum(float v) {
+    v += dpp_or_zero<0x111>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_or_zero<0x112>(v);
+    v += dpp_or_zero<0x114>(v);
+    v += dpp_or_zero<0x118>(v);
+    return v;
+}
+// Lane 63: the sum over the wave
+__device__ __forceinline__ float wave_sum_high(float v) {
+    v = row_sum(v);
+    v += dpp_or_zero<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3
+    v += dpp_or_zero<0x143, 0xc>(v);  // row_bcast 31 into rows 2 and 3
+    return v;
+}
+
 // The slot of row b of a single-token call, or -1: the row is skipped (see fmselective.h). Called by the whole
 // block, for one b: an earlier row with the same slot is looked for by all its threads.
 __device__ __forceinline__ int64_t slot_of_row(const void* __restrict__ slots, bool wide, int32_t b, int64_t S) {

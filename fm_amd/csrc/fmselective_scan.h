@@ -100,19 +100,6 @@ __device__ __forceinline__ void scan_both(float& up_a, float& up_b, float& down_
 
 constexpr int kRowShr1 = 0x111;  // lane i <- lane i-1 inside its row of 16
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_or_zero(float v) {
-    return u2f((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f2u(v), CTRL, 0xf, 0xf, true));
-}
-// Lane 15 of each row of 16: the sum over the row
-__device__ __forceinline__ float row_sum(float v) {
-    v += dpp_or_zero<0x111>(v);
-    v += dpp_or_zero<0x112>(v);
-    v += dpp_or_zero<0x114>(v);
-    v += dpp_or_zero<0x118>(v);
-    return v;
-}
-
 // 8 steps of a row as they lie in memory
 template <typename T>
 struct Raw {
@@ -406,9 +393,9 @@ struct ScanGrads {
 // channel and state A log2 e, the gradient that arrives from later steps, the sum for dA, the state before the tile
 template <int WAVES>
 constexpr size_t scan_sums_bytes() { return (size_t)2 * WAVES * 2 * 256 * sizeof(float); }
-template <int WAVES, int R>
+template <int WAVES>
 size_t scan_backward_lds(int N) {
-    return sizeof(SharedTile<16, 16>) + scan_sums_bytes<WAVES>() + (size_t)WAVES * R * 4 * state_stride(N) * sizeof(float4);
+    return sizeof(SharedTile<16, 16>) + scan_sums_bytes<WAVES>() + (size_t)WAVES * 4 * state_stride(N) * sizeof(float4);
 }
 
 // Backward. The tiles are walked from the last to the first. In a tile the states are made again from the state that
@@ -417,11 +404,11 @@ size_t scan_backward_lds(int N) {
 //   dtokens = dt sum_n dh write + skip g      dA = sum_t dt p      p = dh a h[t-1]
 //   ddt = u sum_n dh write + sum_n A p        dwrite = sum_d dh dt u      dread = sum_d g h
 // The sums over n stay in registers, those over time are added up in LDS, one float a state and channel. The sums
-// over the channels are made in the lane (its R sets of channels), in the wave (4 channels side by side), over the
-// block's waves in LDS and over the blocks by a second kernel, always in the same order.
+// over the channels are made in the wave (4 channels side by side), over the block's waves in LDS and over the
+// blocks by a second kernel, always in the same order.
 // Rows that are too few to fill the GPU are cut into segments, as in forward: the first launch (ENDS) finds what each
 // segment but the first hands on of a gradient that enters it from behind.
-template <typename T, int WAVES, int R, bool ENDS>
+template <typename T, int WAVES, bool ENDS>
 __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, ScanGrads o) {
     constexpr int LPC = 16, NC = 16, kTile = LPC * kSteps;
     using Tile = SharedTile<LPC, NC>;
@@ -432,50 +419,38 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
 
     const Place at = place_of(p);
     const uint32_t b = at.b, g = at.g;
-    const int32_t local = (int32_t)(at.block * WAVES + wave) * 4 * R + ch;  // the lane's first channel; the others follow by fours
-    const int32_t d0 = (int32_t)g * p.per_group + local;
-    const int64_t len = row_length(p.lengths, b, p.L);
-    bool valid[R];
-    int64_t mine[R];
-    float skip[R], bias[R], skip_sum[R], bias_sum[R], all_dt = 0.0f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        valid[r] = local + 4 * r < p.per_group;
-        mine[r] = valid[r] ? len : 0;
-        const int32_t d = valid[r] ? d0 + 4 * r : (int32_t)p.D - 1;
-        skip[r] = p.skip ? param<T>(p.skip, d, p.flags & FMSELECTIVE_NARROW_SKIP) : 0.0f;
-        bias[r] = p.delta_bias ? param<T>(p.delta_bias, d, p.flags & FMSELECTIVE_NARROW_BIAS) : 0.0f;
-        skip_sum[r] = bias_sum[r] = 0.0f;
-    }
-    // (a row beyond the group is addressed but, with no steps that count, never read)
-    const int64_t row = (int64_t)b * p.D + d0;
-    const T* u_row = (const T*)p.tokens + b * p.tokens_b + d0 * p.tokens_d;
-    const T* delta_row = (const T*)p.delta + b * p.delta_b + d0 * p.delta_d;
-    const T* gate_row = p.gate ? (const T*)p.gate + b * p.gate_b + d0 * p.gate_d : nullptr;
-    const T* dy_row = (const T*)o.out_grad + b * o.out_b + d0 * o.out_d;
+    const int32_t local = (int32_t)(at.block * WAVES + wave) * 4 + ch;  // the lane's channel in the group
+    const bool valid = local < p.per_group;
+    const int32_t d = (int32_t)g * p.per_group + (valid ? local : p.per_group - 1);
+    const int64_t row = (int64_t)b * p.D + d;
+    const int64_t len = row_length(p.lengths, b, p.L), mine = valid ? len : 0;
+    const float skip = p.skip ? param<T>(p.skip, d, p.flags & FMSELECTIVE_NARROW_SKIP) : 0.0f;
+    const float bias = p.delta_bias ? param<T>(p.delta_bias, d, p.flags & FMSELECTIVE_NARROW_BIAS) : 0.0f;
+    float skip_sum = 0.0f, bias_sum = 0.0f, all_dt = 0.0f;
+    const T* u_row = (const T*)p.tokens + b * p.tokens_b + d * p.tokens_d;
+    const T* delta_row = (const T*)p.delta + b * p.delta_b + d * p.delta_d;
+    const T* gate_row = p.gate ? (const T*)p.gate + b * p.gate_b + d * p.gate_d : nullptr;
+    const T* dy_row = (const T*)o.out_grad + b * o.out_b + d * o.out_d;
     const T* write_rows = (const T*)p.write + b * p.write_b + g * p.write_g;
     const T* read_rows = (const T*)p.read + b * p.read_b + g * p.read_g;
 
-    const int stride = state_stride(p.N);
-    float4* held = reinterpret_cast<float4*>(lds + sizeof(Tile) + scan_sums_bytes<WAVES>()) + (wave * 4 * R + ch) * stride;
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-        for (int n = c; n < p.N; n += LPC) {
-            float e = 0.0f, rate = 0.0f;
-            if (valid[r]) {
-                const int64_t at_n = (row + 4 * r) * p.N + n;
-                rate = p.A[(int64_t)(d0 + 4 * r) * p.N + n] * kLog2E;
-                if (!ENDS) {
-                    if (o.final_grad) e = o.final_grad[at_n];
+    float4* held = reinterpret_cast<float4*>(lds + sizeof(Tile) + scan_sums_bytes<WAVES>()) + (wave * 4 + ch) * state_stride(p.N);
+    for (int n = c; n < p.N; n += LPC) {
+        float e = 0.0f, rate = 0.0f;
+        if (valid) {
+            const int64_t at_n = row * p.N + n;
+            rate = p.A[(int64_t)d * p.N + n] * kLog2E;
+            if (!ENDS) {
+                if (o.final_grad) e = o.final_grad[at_n];
 #pragma unroll 4
-                    for (int32_t j = p.segments - 1; j > at.seg; --j) {
-                        const float2 q = p.pairs[j * p.rows * p.N + at_n];
-                        e = __builtin_fmaf(q.x, e, q.y);
-                    }
+                for (int32_t j = p.segments - 1; j > at.seg; --j) {
+                    const float2 q = p.pairs[j * p.rows * p.N + at_n];
+                    e = __builtin_fmaf(q.x, e, q.y);
                 }
             }
-            held[4 * r * stride + n] = make_float4(rate, e, 0.0f, 0.0f);
         }
+        held[n] = make_float4(rate, e, 0.0f, 0.0f);
+    }
 
     const int chunks = (p.N + NC - 1) / NC;
     const int32_t row_tiles = (int32_t)((len + kTile - 1) / kTile), first_tile = at.seg * p.seg_tiles;
@@ -491,35 +466,32 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
     for (int32_t tile = n_tiles - 1; tile >= first_tile; --tile) {
         const int64_t t0 = (int64_t)tile * kTile + c * kSteps;
         const bool ragged = (int64_t)(tile + 1) * kTile > len;
-        float dt[R][kSteps], dtu[R][kSteps], gy[R][kSteps], sum_w[R][kSteps], sum_a[R][kSteps], y[R][kSteps], total_dt[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const Raw<T> raw_d = load_raw<T>(delta_row + 4 * r * p.delta_d, t0, mine[r]),
-                         raw_g = load_raw<T>(dy_row + 4 * r * o.out_d, t0, mine[r]);
+        const int left = ragged ? steps_left(mine, t0) : kSteps;
+        float dt[kSteps], dtu[kSteps], gy[kSteps], sum_w[kSteps], sum_a[kSteps], y[kSteps], total_dt = 0.0f;
+        {
+            const Raw<T> raw_d = load_raw<T>(delta_row, t0, mine), raw_g = load_raw<T>(dy_row, t0, mine);
             Raw<T> raw_u = {}, raw_z = {};
-            if (!ENDS) raw_u = load_raw<T>(u_row + 4 * r * p.tokens_d, t0, mine[r]);
-            if (gate_row) raw_z = load_raw<T>(gate_row + 4 * r * p.gate_d, t0, mine[r]);
+            if (!ENDS) raw_u = load_raw<T>(u_row, t0, mine);
+            if (gate_row) raw_z = load_raw<T>(gate_row, t0, mine);
             if (!ENDS)
-                for (int n = c; n < p.N; n += LPC)
-                    held[4 * r * stride + n].w = valid[r] ? o.marks[((row + 4 * r) * p.marks + tile) * p.N + n] : 0.0f;
+                for (int n = c; n < p.N; n += LPC) held[n].w = valid ? o.marks[(row * p.marks + tile) * p.N + n] : 0.0f;
             float u[kSteps], z[kSteps];
-            widen_raw(raw_d, dt[r]);
-            widen_raw(raw_g, gy[r]);
-            steps_of(dt[r], bias[r], p.flags, ragged, ragged ? steps_left(mine[r], t0) : kSteps);
+            widen_raw(raw_d, dt);
+            widen_raw(raw_g, gy);
+            steps_of(dt, bias, p.flags, ragged, left);
             if (gate_row) {
                 widen_raw(raw_z, z);
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) gy[r][k] *= z[k] * sigmoid(z[k]);
+                for (int k = 0; k < kSteps; ++k) gy[k] *= z[k] * sigmoid(z[k]);
             }
             widen_raw(raw_u, u);
-            total_dt[r] = 0.0f;
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
-                dtu[r][k] = dt[r][k] * u[k];
-                total_dt[r] += dt[r][k];
-                sum_w[r][k] = sum_a[r][k] = y[r][k] = 0.0f;
+                dtu[k] = dt[k] * u[k];
+                total_dt += dt[k];
+                sum_w[k] = sum_a[k] = y[k] = 0.0f;
             }
-            if (ENDS) all_dt += total_dt[r];
+            if (ENDS) all_dt += total_dt;
         }
         for (int chunk = 0; chunk < chunks; ++chunk) {
             loader.put(shared);
@@ -533,64 +505,53 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
                 float w[kSteps], rd[kSteps];
                 if (!ENDS) steps_at<LPC>(steps, w);
                 steps_at<LPC>(steps + NC * 8 * LPC, rd);
-                float write_terms[kSteps], read_terms[kSteps];
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    float4& mem = state[4 * r * stride];
-                    const float4 e = mem;
-                    float a[kSteps], h[kSteps], dh[kSteps];
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        a[k] = exp2_fast(dt[r][k] * e.x);
-                        dh[k] = rd[k] * gy[r][k];
-                        if (!ENDS) h[k] = w[k] * dtu[r][k];
-                    }
-                    float S = 0.0f, P = exp2_fast(total_dt[r] * e.x), D = dh[kSteps - 1], Q = P;
-#pragma unroll
-                    for (int k = kSteps - 1; k > 0; --k) D = __builtin_fmaf(a[k], D, dh[k - 1]);
-                    D *= a[0];
-                    if constexpr (ENDS) {
-                        scan_down(Q, D);
-                        if (c == 0) mem.y = __builtin_fmaf(Q, e.y, D);
-                        continue;
-                    }
-                    S = h[0];
-#pragma unroll
-                    for (int k = 1; k < kSteps; ++k) S = __builtin_fmaf(a[k], S, h[k]);
-                    scan_both(P, S, Q, D);
-                    const float enter = __builtin_fmaf(fmscan::dpp<kRowShr1>(1.0f, P), e.w, fmscan::dpp<kRowShr1>(0.0f, S));
-                    float back = __builtin_fmaf(fmscan::dpp<fmscan::kRowShl1>(1.0f, Q), e.y, fmscan::dpp<fmscan::kRowShl1>(0.0f, D));
-                    if (c == 0) mem.y = __builtin_fmaf(Q, e.y, D);
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        h[k] = __builtin_fmaf(a[k], k ? h[k - 1] : enter, h[k]);
-                        y[r][k] = __builtin_fmaf(rd[k], h[k], y[r][k]);
-                        read_terms[k] = r ? __builtin_fmaf(gy[r][k], h[k], read_terms[k]) : gy[r][k] * h[k];
-                    }
-                    float in_time = 0.0f;
-#pragma unroll
-                    for (int k = kSteps - 1; k >= 0; --k) {
-                        dh[k] += back;
-                        back = a[k] * dh[k];
-                        const float pk = back * (k ? h[k - 1] : enter);
-                        sum_w[r][k] = __builtin_fmaf(dh[k], w[k], sum_w[r][k]);
-                        sum_a[r][k] = __builtin_fmaf(e.x, pk, sum_a[r][k]);
-                        in_time = __builtin_fmaf(dt[r][k], pk, in_time);
-                        write_terms[k] = r ? __builtin_fmaf(dh[k], dtu[r][k], write_terms[k]) : dh[k] * dtu[r][k];
-                    }
-                    in_time = row_sum(in_time);
-                    if (c == 15) mem.z = e.z + in_time;
-                }
-                if constexpr (ENDS) continue;
-                // The 4 channels side by side: a swap exchanges halves of two registers, so that one addition settles
-                // both. First the halves of the wave (lanes below 32 keep write's sums, the others read's), then
-                // the rows of a half (the even one keeps steps 0 to 3, the odd one 4 to 7).
-                float half[kSteps];
+                const float4 e = *state;
+                float a[kSteps], h[kSteps], dh[kSteps];
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
-                    const auto s = __builtin_amdgcn_permlane32_swap(f2u(write_terms[k]), f2u(read_terms[k]), false, false);
+                    a[k] = exp2_fast(dt[k] * e.x);
+                    dh[k] = rd[k] * gy[k];
+                    if (!ENDS) h[k] = w[k] * dtu[k];
+                }
+                float S = 0.0f, P = exp2_fast(total_dt * e.x), D = dh[kSteps - 1], Q = P;
+#pragma unroll
+                for (int k = kSteps - 1; k > 0; --k) D = __builtin_fmaf(a[k], D, dh[k - 1]);
+                D *= a[0];
+                if constexpr (ENDS) {
+                    scan_down(Q, D);
+                    if (c == 0) state->y = __builtin_fmaf(Q, e.y, D);
+                    continue;
+                }
+                S = h[0];
+#pragma unroll
+                for (int k = 1; k < kSteps; ++k) S = __builtin_fmaf(a[k], S, h[k]);
+                scan_both(P, S, Q, D);
+                const float enter = __builtin_fmaf(fmscan::dpp<kRowShr1>(1.0f, P), e.w, fmscan::dpp<kRowShr1>(0.0f, S));
+                float back = __builtin_fmaf(fmscan::dpp<fmscan::kRowShl1>(1.0f, Q), e.y, fmscan::dpp<fmscan::kRowShl1>(0.0f, D));
+                if (c == 0) state->y = __builtin_fmaf(Q, e.y, D);
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    h[k] = __builtin_fmaf(a[k], k ? h[k - 1] : enter, h[k]);
+                    y[k] = __builtin_fmaf(rd[k], h[k], y[k]);
+                }
+                float in_time = 0.0f, half[kSteps];
+#pragma unroll
+                for (int k = kSteps - 1; k >= 0; --k) {
+                    dh[k] += back;
+                    back = a[k] * dh[k];
+                    const float pk = back * (k ? h[k - 1] : enter);
+                    sum_w[k] = __builtin_fmaf(dh[k], w[k], sum_w[k]);
+                    sum_a[k] = __builtin_fmaf(e.x, pk, sum_a[k]);
+                    in_time = __builtin_fmaf(dt[k], pk, in_time);
+                    // The 4 channels side by side: a swap exchanges halves of two registers, so that one addition
+                    // settles both. First the halves of the wave: lanes below 32 keep write's sums, the others
+                    // read's.
+                    const auto s = __builtin_amdgcn_permlane32_swap(f2u(dh[k] * dtu[k]), f2u(gy[k] * h[k]), false, false);
                     half[k] = u2f(s[0]) + u2f(s[1]);
                 }
+                in_time = row_sum(in_time);
+                if (c == 15) state->z = e.z + in_time;
+                // then the rows of a half: the even one keeps steps 0 to 3, the odd one 4 to 7
                 float4 row_sums;
                 float* q = &row_sums.x;
 #pragma unroll
@@ -623,53 +584,47 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
             __syncthreads();  // the tile may be filled again
         }
         if (ENDS) continue;
+        float u[kSteps], dd[kSteps], x[kSteps], z[kSteps];
+        load_values<T, kSteps>(u_row, t0, mine, u);
+        load_values<T, kSteps>(delta_row, t0, mine, x);
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int64_t at_row = (row + 4 * r) * p.L;
-            const int left = ragged ? steps_left(mine[r], t0) : kSteps;
-            float u[kSteps], dd[kSteps], x[kSteps], z[kSteps];
-            load_values<T, kSteps>(u_row + 4 * r * p.tokens_d, t0, mine[r], u);
-            load_values<T, kSteps>(delta_row + 4 * r * p.delta_d, t0, mine[r], x);
+        for (int k = 0; k < kSteps; ++k) {
+            dd[k] = __builtin_fmaf(u[k], sum_w[k], kLn2 * sum_a[k]);
+            if (p.flags & FMSELECTIVE_SOFTPLUS) dd[k] *= sigmoid(x[k] + bias);
+            x[k] = __builtin_fmaf(dt[k], sum_w[k], skip * gy[k]);
+            y[k] = __builtin_fmaf(skip, u[k], y[k]);
+        }
+        if (ragged) {
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
-                dd[k] = __builtin_fmaf(u[k], sum_w[r][k], kLn2 * sum_a[r][k]);
-                if (p.flags & FMSELECTIVE_SOFTPLUS) dd[k] *= sigmoid(x[k] + bias[r]);
-                x[k] = __builtin_fmaf(dt[r][k], sum_w[r][k], skip[r] * gy[r][k]);
-                y[r][k] = __builtin_fmaf(skip[r], u[k], y[r][k]);
+                dd[k] = k < left ? dd[k] : 0.0f;
+                x[k] = k < left ? x[k] : 0.0f;
             }
+        }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            bias_sum += dd[k];
+            skip_sum = __builtin_fmaf(gy[k], u[k], skip_sum);
+        }
+        if (valid) {
+            store_values<T, kSteps>((T*)o.tokens + row * p.L, t0, p.L, x);
+            store_values<T, kSteps>((T*)o.delta + row * p.L, t0, p.L, dd);
+        }
+        if (gate_row) {
+            load_values<T, kSteps>(dy_row, t0, mine, dd);
+            load_values<T, kSteps>(gate_row, t0, mine, z);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) dd[k] *= y[k] * silu_slope(z[k], sigmoid(z[k]));
             if (ragged) {
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    dd[k] = k < left ? dd[k] : 0.0f;
-                    x[k] = k < left ? x[k] : 0.0f;
-                }
+                for (int k = 0; k < kSteps; ++k) dd[k] = k < left ? dd[k] : 0.0f;
             }
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                bias_sum[r] += dd[k];
-                skip_sum[r] = __builtin_fmaf(gy[r][k], u[k], skip_sum[r]);
-            }
-            if (valid[r]) {
-                store_values<T, kSteps>((T*)o.tokens + at_row, t0, p.L, x);
-                store_values<T, kSteps>((T*)o.delta + at_row, t0, p.L, dd);
-            }
-            if (gate_row) {
-                load_values<T, kSteps>(dy_row + 4 * r * o.out_d, t0, mine[r], dd);
-                load_values<T, kSteps>(gate_row + 4 * r * p.gate_d, t0, mine[r], z);
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) dd[k] *= y[r][k] * silu_slope(z[k], sigmoid(z[k]));
-                if (ragged) {
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) dd[k] = k < left ? dd[k] : 0.0f;
-                }
-                if (valid[r]) store_values<T, kSteps>((T*)o.gate + at_row, t0, p.L, dd);
-            }
+            if (valid) store_values<T, kSteps>((T*)o.gate + row * p.L, t0, p.L, dd);
         }
     }
     if constexpr (ENDS) {
-        static_assert(!ENDS || R == 1, "one set of channels");
         all_dt = __shfl(row_sum(all_dt), lane | 15);
-        if (valid[0])
+        if (valid)
             for (int n = c; n < p.N; n += LPC)
                 p.pairs[((int64_t)at.seg * p.rows + row) * p.N + n] = make_float2(exp2_fast(all_dt * held[n].x), held[n].y);
         return;
@@ -677,28 +632,23 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
     float zero[kSteps];
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) zero[k] = 0.0f;
+    skip_sum = row_sum(skip_sum);
+    bias_sum = row_sum(bias_sum);
+    if (!valid) return;
     const int64_t end = (int64_t)seg_end * kTile < p.L ? (int64_t)seg_end * kTile : p.L;
+    for (int64_t t0 = (int64_t)(n_tiles > first_tile ? n_tiles : first_tile) * kTile + c * kSteps; t0 < end; t0 += kTile) {
+        store_values<T, kSteps>((T*)o.tokens + row * p.L, t0, p.L, zero);
+        store_values<T, kSteps>((T*)o.delta + row * p.L, t0, p.L, zero);
+        if (gate_row) store_values<T, kSteps>((T*)o.gate + row * p.L, t0, p.L, zero);
+    }
     const int64_t part_row = (int64_t)at.seg * p.rows + row;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        skip_sum[r] = row_sum(skip_sum[r]);
-        bias_sum[r] = row_sum(bias_sum[r]);
-        if (!valid[r]) continue;
-        const int64_t at_row = (row + 4 * r) * p.L;
-        for (int64_t t0 = (int64_t)(n_tiles > first_tile ? n_tiles : first_tile) * kTile + c * kSteps; t0 < end; t0 += kTile) {
-            store_values<T, kSteps>((T*)o.tokens + at_row, t0, p.L, zero);
-            store_values<T, kSteps>((T*)o.delta + at_row, t0, p.L, zero);
-            if (gate_row) store_values<T, kSteps>((T*)o.gate + at_row, t0, p.L, zero);
-        }
-        if (c == 15) {
-            if (o.skip_part) o.skip_part[part_row + 4 * r] = skip_sum[r];
-            if (o.bias_part) o.bias_part[part_row + 4 * r] = bias_sum[r];
-        }
-        for (int n = c; n < p.N; n += LPC) {
-            const float4 e = held[4 * r * stride + n];
-            o.A_part[(part_row + 4 * r) * p.N + n] = e.z;
-            if (o.initial && at.seg == 0) o.initial[(row + 4 * r) * p.N + n] = e.y;
-        }
+    if (c == 15) {
+        if (o.skip_part) o.skip_part[part_row] = skip_sum;
+        if (o.bias_part) o.bias_part[part_row] = bias_sum;
+    }
+    for (int n = c; n < p.N; n += LPC) {
+        o.A_part[part_row * p.N + n] = held[n].z;
+        if (o.initial && at.seg == 0) o.initial[row * p.N + n] = held[n].y;
     }
 }
 

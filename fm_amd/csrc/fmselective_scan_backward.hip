@@ -9,11 +9,7 @@ namespace {
 
 constexpr int kBackWaves = fmselective::kScanWaves;
 
-// Sets of channels a lane works on: two where that leaves two waves a SIMD, which halves the additions over
-// channels and the partial sums in memory; one otherwise, with the rows cut where those are too few.
-#ifndef FMSELECTIVE_BACK_TWO
-#define FMSELECTIVE_BACK_TWO 2048
-#endif
+// The rows are cut where they leave too few waves.
 #ifndef FMSELECTIVE_BACK_CUT_BELOW
 #define FMSELECTIVE_BACK_CUT_BELOW 1024
 #endif
@@ -21,17 +17,14 @@ constexpr int kBackWaves = fmselective::kScanWaves;
 #define FMSELECTIVE_BACK_CUT_WANT 2048
 #endif
 struct BackPlan {
-    int sets;
     Cut cut;
     int64_t blocks, shared, states, rows, pairs;  // blocks; floats of the partial sums and of the pairs
     size_t bytes() const { return (size_t)(shared + pairs + states + 2 * rows) * sizeof(float); }
 };
 BackPlan plan_backward(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) {
     const int64_t per_group = D / G, marks = (L + fmselective::kMark - 1) / fmselective::kMark;
-    auto blocks = [&](int sets) { return B * G * ((per_group + 4 * kBackWaves * sets - 1) / (4 * kBackWaves * sets)); };
     BackPlan b;
-    b.sets = blocks(2) * kBackWaves >= FMSELECTIVE_BACK_TWO ? 2 : 1;
-    b.blocks = blocks(b.sets);
+    b.blocks = B * G * ((per_group + 4 * kBackWaves - 1) / (4 * kBackWaves));
     const int64_t waves = b.blocks * kBackWaves;
     b.cut = cut_of(marks, waves, waves < FMSELECTIVE_BACK_CUT_BELOW ? FMSELECTIVE_BACK_CUT_WANT : waves);
     b.shared = b.blocks * N * marks * 256;
@@ -41,11 +34,11 @@ BackPlan plan_backward(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) {
     return b;
 }
 
-template <typename T, int R, bool ENDS>
+template <typename T, bool ENDS>
 int launch_backward(const char* who, const Scan& p, const ScanGrads& g, int64_t blocks, hipStream_t stream) {
     static std::atomic<uint64_t> armed{0};
-    const size_t lds = fmselective::scan_backward_lds<kBackWaves, R>(p.N);
-    const auto kernel = fmselective::selective_backward_kernel<T, kBackWaves, R, ENDS>;
+    const size_t lds = fmselective::scan_backward_lds<kBackWaves>(p.N);
+    const auto kernel = fmselective::selective_backward_kernel<T, kBackWaves, ENDS>;
     if (lds > 64 * 1024)
         if (int rc = raise_lds_limit((const void*)kernel, armed, who)) return rc;
     kernel<<<(unsigned)blocks, 64 * kBackWaves, lds, stream>>>(p, g);
@@ -97,7 +90,7 @@ int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselecti
             if (&q != &r && overlap(q, r)) return fail(FMSCAN_E_ALIAS, "%s: %s overlaps %s", who, r.name, q.name);
     }
     float* const pairs = (float*)workspace + b.shared;
-    const Scan p = scan_of(*in, 4 * kBackWaves * b.sets, b.cut, pairs);
+    const Scan p = scan_of(*in, 4 * kBackWaves, b.cut, pairs);
     const int64_t lines = in->B * in->G * in->N, waves = lines * p.marks, blocks = b.blocks * b.cut.segments;
     if (blocks > INT32_MAX || waves > (int64_t)INT32_MAX * 4)
         return fail(FMSCAN_E_SHAPE, "%s: B * D or B * G * N * L is too large for one launch", who);
@@ -120,9 +113,8 @@ int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselecti
     with_dtype(in->dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
         const hipStream_t st = (hipStream_t)stream;
-        if (b.cut.segments > 1 && (rc = launch_backward<T, 1, true>(who, p, g, blocks, st))) return;
-        rc = b.sets == 2 ? launch_backward<T, 2, false>(who, p, g, blocks, st) : launch_backward<T, 1, false>(who, p, g, blocks, st);
-        if (rc) return;
+        if (b.cut.segments > 1 && (rc = launch_backward<T, true>(who, p, g, blocks, st))) return;
+        if ((rc = launch_backward<T, false>(who, p, g, blocks, st))) return;
         fmselective::selective_shared_grads_kernel<T><<<(unsigned)((waves + 3) / 4), 256, 0, (hipStream_t)stream>>>(
             part, (T*)o.write, (T*)o.read, in->lengths, in->L, waves, p.N, p.G, p.marks, p.blocks_per_group);
         rc = launched("selective scan (gradients of write and read)");
