@@ -365,7 +365,53 @@ __global__ __launch_bounds__(256) void conv_backward_kernel(const T* __restrict_
     if (live && c == 0) bias_part[at] = db;
 }
 
-// One token: a thread a channel of a row. The state moves by one place and takes the new input.
+// 4 M consecutive values as M accesses at the alignment of an element, those from `count` on untouched
+template <typename T, int M>
+__device__ __forceinline__ void load_fours(const T* p, int count, T (&f)[4 * M]) {
+    typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (count >= 4 * M) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const four v = reinterpret_cast<const four*>(p)[i];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[4 * i + k] = v[k];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4 * M; ++i) f[i] = i < count ? p[i] : (T)0.0f;
+    }
+}
+template <typename T, int M>
+__device__ __forceinline__ void store_fours(T* p, int count, const T (&f)[4 * M]) {
+    typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (count >= 4 * M) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            four v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = f[4 * i + k];
+            reinterpret_cast<four*>(p)[i] = v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4 * M; ++i)
+            if (i < count) p[i] = f[i];
+    }
+}
+template <typename T, int M>
+__device__ __forceinline__ void load_param_fours(const void* p, int64_t at, bool narrow, int count, float (&f)[4 * M]) {
+    if (narrow) {
+        T v[4 * M];
+        load_fours<T, M>(reinterpret_cast<const T*>(p) + at, count, v);
+#pragma unroll
+        for (int i = 0; i < 4 * M; ++i) f[i] = Elem<T>::widen(v[i]);
+    } else {
+        load_fours<float, M>(reinterpret_cast<const float*>(p) + at, count, f);
+    }
+}
+
+// One token: four channels of a row a thread, whose states are 4 (W - 1) values in a row. The state moves by one place
+// and takes the new input.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void conv_step_kernel(const T* __restrict__ inputs, int64_t batch_stride, const T* state,
                                                         T* state_out, const void* __restrict__ weight,
@@ -373,26 +419,37 @@ __global__ __launch_bounds__(256) void conv_step_kernel(const T* __restrict__ in
                                                         T* __restrict__ out, int32_t D, uint32_t tiles, int64_t S,
                                                         unsigned flags) {
     const uint32_t b = tiles == 1 ? blockIdx.x : blockIdx.x / tiles;
-    const int64_t d = (int64_t)(blockIdx.x - b * tiles) * blockDim.x + threadIdx.x;
-    const int64_t slot = slot_of_row(slots, flags & FMSELECTIVE_SLOTS_64, (int32_t)b, S);
-    if (d >= D) return;
-    if (slot < 0) {
-        out[(int64_t)b * D + d] = (T)0.0f;
-        return;
+    const int32_t d = ((blockIdx.x - b * tiles) * blockDim.x + threadIdx.x) * 4;
+    const int n = D - d;  // channels left, this thread's among them
+    T x[4];
+    float w[4 * W], v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (n > 0) {
+        load_fours<T, 1>(inputs + b * batch_stride + d, n, x);
+        load_param_fours<T, W>(weight, (int64_t)d * W, flags & FMSELECTIVE_NARROW_WEIGHT, n < 4 ? n * W : 4 * W, w);
+        if (bias) load_param_fours<T, 1>(bias, d, flags & FMSELECTIVE_NARROW_BIAS, n, v);
     }
-    const int64_t at = (slot * D + d) * (W - 1);
-    T window[W];
+    const int64_t slot = slot_of_row(slots, flags & FMSELECTIVE_SLOTS_64, (int32_t)b, S);
+    if (n <= 0) return;
+    T y[4] = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
+    if (slot >= 0) {
+        const int64_t at = (slot * D + d) * (W - 1);
+        const int held = n < 4 ? n * (W - 1) : 4 * (W - 1);
+        T old[4 * (W - 1)], moved[4 * (W - 1)];
+        load_fours<T, W - 1>(state + at, held, old);
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) window[j] = state[at + j];
-    window[W - 1] = inputs[b * batch_stride + d];
-    float w[W], v;
-    conv_taps<T, W>(weight, bias, d, flags, w, v);
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) v = __builtin_fmaf(w[j], Elem<T>::widen(window[j]), v);
-    if (flags & FMSELECTIVE_SILU) v *= sigmoid(v);
-    out[(int64_t)b * D + d] = (T)v;
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j) state_out[at + j] = window[j + 1];
+            for (int j = 0; j < W; ++j) {
+                const T value = j < W - 1 ? old[i * (W - 1) + (j < W - 1 ? j : 0)] : x[i];
+                v[i] = __builtin_fmaf(w[i * W + j], Elem<T>::widen(value), v[i]);
+                if (j) moved[i * (W - 1) + (j ? j - 1 : 0)] = value;
+            }
+            if (flags & FMSELECTIVE_SILU) v[i] *= sigmoid(v[i]);
+            y[i] = (T)v[i];
+        }
+        store_fours<T, W - 1>(state_out + at, held, moved);
+    }
+    store_fours<T, 1>(out + (int64_t)b * D + d, n, y);
 }
 
 }  // namespace fmselective

@@ -173,7 +173,7 @@ int fmselective_conv_step(const void* inputs, int64_t batch_stride, const void* 
     if (int rc = check_alias(who, {out_r}, {old_r})) return rc;
     if (state_out != state)
         if (int rc = check_alias(who, {new_r}, {old_r})) return rc;
-    const uint32_t tiles = (uint32_t)((D + 255) / 256);
+    const uint32_t tiles = (uint32_t)((D + 1023) / 1024);
     if ((__int128)B * tiles > (__int128)INT32_MAX) return fail(FMSCAN_E_SHAPE, "%s: B * D is too large for one launch", who);
     with_dtype(dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;

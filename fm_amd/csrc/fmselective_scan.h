@@ -98,6 +98,8 @@ __device__ __forceinline__ void scan_both(float& up_a, float& up_b, float& down_
 }
 #undef FMSELECTIVE_LEVEL
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kRowShr1 = 0x111;  // lane i <- lane i-1 inside its row of 16
 
 // 8 steps of a row as they lie in memory
@@ -694,66 +696,93 @@ struct Step {
 };
 
 // One token: four lanes a channel, each takes every fourth group of four states, 16 bytes at a time where N allows;
-// a block takes 64 channels of a row.
-template <typename T, bool VEC>
+// a block takes 64 channels of a row, CH times. The row's `write` and `read` serve all its channels of a group.
+// Bound by the pool's traffic: what does not depend on the slot is loaded before it is known, and with CH = 4 a lane
+// has four states' loads in flight.
+template <typename T, bool VEC, int CH>
 __global__ __launch_bounds__(256) void selective_step_kernel(Step p, T* __restrict__ out) {
     const uint32_t b = p.tiles == 1 ? blockIdx.x : blockIdx.x / p.tiles;
-    const int64_t d = (int64_t)(blockIdx.x - b * p.tiles) * 64 + threadIdx.x / 4;
+    const int64_t first = (int64_t)(blockIdx.x - b * p.tiles) * (64 * CH) + threadIdx.x / 4;
     const int part = threadIdx.x & 3;
+    float u[CH], dt[CH], z[CH], skip[CH], y[CH];
+    int32_t g[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int64_t d = first + 64 * i < p.D ? first + 64 * i : p.D - 1;  // (a lane beyond the last channel repeats it)
+        u[i] = Elem<T>::widen(((const T*)p.tokens)[b * p.tokens_b + d]);
+        dt[i] = Elem<T>::widen(((const T*)p.delta)[b * p.delta_b + d]);
+        z[i] = p.gate ? Elem<T>::widen(((const T*)p.gate)[b * p.gate_b + d]) : 0.0f;
+        if (p.delta_bias) dt[i] += param<T>(p.delta_bias, d, p.flags & FMSELECTIVE_NARROW_BIAS);
+        skip[i] = p.skip ? param<T>(p.skip, d, p.flags & FMSELECTIVE_NARROW_SKIP) : 0.0f;
+        g[i] = p.per_group == p.D ? 0 : (int32_t)d / p.per_group;
+        y[i] = 0.0f;
+    }
     const int64_t slot = slot_of_row(p.slots, p.flags & FMSELECTIVE_SLOTS_64, (int32_t)b, p.S);
-    if (d >= p.D) return;  // whole groups of four lanes
     if (slot < 0) {
-        if (part == 0) out[(int64_t)b * p.D + d] = (T)0.0f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (part == 0 && first + 64 * i < p.D) out[(int64_t)b * p.D + first + 64 * i] = (T)0.0f;
         return;
     }
-    const int32_t g = (int32_t)d / p.per_group;
-    const float u = Elem<T>::widen(((const T*)p.tokens)[b * p.tokens_b + d]);
-    float dt = Elem<T>::widen(((const T*)p.delta)[b * p.delta_b + d]);
-    if (p.delta_bias) dt += param<T>(p.delta_bias, d, p.flags & FMSELECTIVE_NARROW_BIAS);
-    if (p.flags & FMSELECTIVE_SOFTPLUS) dt = softplus(dt);
-    const float dtu = dt * u;
-    const T* write = (const T*)p.write + b * p.write_b + g * p.write_g;
-    const T* read = (const T*)p.read + b * p.read_b + g * p.read_g;
-    const float* A = p.A + d * p.N;
-    const float* state = p.state + (slot * p.D + d) * p.N;
-    float* state_out = p.state_out + (slot * p.D + d) * p.N;
-    float y = 0.0f;
-    for (int n0 = part * 4; n0 < p.N; n0 += 16) {
-        float a[4], h[4];
-        if constexpr (VEC) {  // N is a multiple of 4, the pools and A lie on 16 bytes
-            *reinterpret_cast<float4*>(a) = *reinterpret_cast<const float4*>(A + n0);
-            *reinterpret_cast<float4*>(h) = *reinterpret_cast<const float4*>(state + n0);
-        } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool in = n0 + k < p.N;
-                a[k] = in ? A[n0 + k] : 0.0f;
-                h[k] = in ? state[n0 + k] : 0.0f;
+    for (int i = 0; i < CH; ++i)
+        if (p.flags & FMSELECTIVE_SOFTPLUS) dt[i] = softplus(dt[i]);
+    const T* write = (const T*)p.write + b * p.write_b;
+    const T* read = (const T*)p.read + b * p.read_b;
+    const float* state = p.state + slot * p.D * p.N;
+    float* state_out = p.state_out + slot * p.D * p.N;
+    for (int n0 = part * 4; n0 < p.N; n0 += 16) {
+        float a[CH][4], h[CH][4], w[4], r[4];
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int64_t d = first + 64 * i < p.D ? first + 64 * i : p.D - 1;
+            if constexpr (VEC) {  // N is a multiple of 4, the pools and A lie on 16 bytes
+                *reinterpret_cast<f32x4*>(h[i]) = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(state + d * p.N + n0));
+                *reinterpret_cast<f32x4*>(a[i]) = *reinterpret_cast<const f32x4*>(p.A + d * p.N + n0);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const bool in = n0 + k < p.N;
+                    h[i][k] = in ? state[d * p.N + n0 + k] : 0.0f;
+                    a[i][k] = in ? p.A[d * p.N + n0 + k] : 0.0f;
+                }
             }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (!VEC && n0 + k >= p.N) continue;
-            h[k] = __builtin_fmaf(exp2_fast(dt * (a[k] * kLog2E)), h[k], dtu * Elem<T>::widen(write[n0 + k]));
-            y = __builtin_fmaf(Elem<T>::widen(read[n0 + k]), h[k], y);
-        }
-        if constexpr (VEC) {
-            *reinterpret_cast<float4*>(state_out + n0) = *reinterpret_cast<float4*>(h);
-        } else {
+        for (int i = 0; i < CH; ++i) {
+            if (i == 0 || g[i] != g[i ? i - 1 : 0]) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (n0 + k < p.N) state_out[n0 + k] = h[k];
+                for (int k = 0; k < 4; ++k) {
+                    const bool in = VEC || n0 + k < p.N;
+                    w[k] = in ? Elem<T>::widen(write[g[i] * p.write_g + n0 + k]) : 0.0f;
+                    r[k] = in ? Elem<T>::widen(read[g[i] * p.read_g + n0 + k]) : 0.0f;
+                }
+            }
+            const float dtu = dt[i] * u[i];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                h[i][k] = __builtin_fmaf(exp2_fast(dt[i] * (a[i][k] * kLog2E)), h[i][k], dtu * w[k]);
+                y[i] = __builtin_fmaf(r[k], h[i][k], y[i]);
+            }
+            const int64_t d = first + 64 * i;
+            if (d >= p.D) continue;
+            if constexpr (VEC) {
+                __builtin_nontemporal_store(*reinterpret_cast<f32x4*>(h[i]), reinterpret_cast<f32x4*>(state_out + d * p.N + n0));
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (n0 + k < p.N) state_out[d * p.N + n0 + k] = h[i][k];
+            }
         }
     }
-    y += fmscan::dpp<0xb1>(0.0f, y);  // quad_perm 1,0,3,2
-    y += fmscan::dpp<0x4e>(0.0f, y);  // quad_perm 2,3,0,1
-    if (part) return;
-    if (p.skip) y = __builtin_fmaf(param<T>(p.skip, d, p.flags & FMSELECTIVE_NARROW_SKIP), u, y);
-    if (p.gate) {
-        const float z = Elem<T>::widen(((const T*)p.gate)[b * p.gate_b + d]);
-        y *= z * sigmoid(z);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        y[i] += fmscan::dpp<0xb1>(0.0f, y[i]);  // quad_perm 1,0,3,2
+        y[i] += fmscan::dpp<0x4e>(0.0f, y[i]);  // quad_perm 2,3,0,1
+        if (p.skip) y[i] = __builtin_fmaf(skip[i], u[i], y[i]);
+        if (p.gate) y[i] *= z[i] * sigmoid(z[i]);
+        if (part == 0 && first + 64 * i < p.D) out[(int64_t)b * p.D + first + 64 * i] = (T)y[i];
     }
-    out[(int64_t)b * p.D + d] = (T)y;
 }
 
 }  // namespace fmselective

@@ -20,6 +20,9 @@ namespace {
 #ifndef FMSELECTIVE_WAVES64
 #define FMSELECTIVE_WAVES64 8
 #endif
+// A single token's call: blocks of 64 channels from which on a block takes 256 instead
+constexpr int64_t kManyStepBlocks = 4096;
+
 struct ForwardPlan {
     int lanes;
     Cut cut;
@@ -137,14 +140,17 @@ int fmselective_scan_step(const fmselective_scan_inputs* in, float* state_out, c
     p.read_b = in->read_strides[0]; p.read_g = in->read_strides[1];
     p.S = S;
     p.D = (int32_t)D; p.N = (int32_t)in->N; p.per_group = (int32_t)(D / in->G);
-    p.tiles = (uint32_t)((D + 63) / 64);
+    const bool many = B * ((D + 63) / 64) >= kManyStepBlocks;
+    p.tiles = (uint32_t)(many ? (D + 255) / 256 : (D + 63) / 64);
     p.flags = in->flags;
     if ((__int128)B * p.tiles > (__int128)INT32_MAX) return fail(FMSCAN_E_SHAPE, "%s: B * D is too large for one launch", who);
     const bool vec = in->N % 4 == 0 && aligned16(in->A) && aligned16(in->initial_state) && aligned16(state_out);
     with_dtype(in->dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
         with_bool(vec, [&](auto vt) {
-            fmselective::selective_step_kernel<T, decltype(vt)::value><<<(unsigned)(B * p.tiles), 256, 0, (hipStream_t)stream>>>(p, (T*)out);
+            constexpr bool VEC = decltype(vt)::value;
+            const auto kernel = many ? fmselective::selective_step_kernel<T, VEC, 4> : fmselective::selective_step_kernel<T, VEC, 1>;
+            kernel<<<(unsigned)(B * p.tiles), 256, 0, (hipStream_t)stream>>>(p, (T*)out);
         });
     });
     return launched("selective scan (one token)");
