@@ -117,14 +117,14 @@ struct ColumnSums {
 constexpr int kSumWaves = 16;
 
 template <typename T>
-__global__ __launch_bounds__(64 * kSumWaves) void column_sums_kernel(ColumnSums s) {
+__device__ __forceinline__ void column_sums(const ColumnSums& s, uint32_t block) {
     int which = 0;
 #pragma unroll
     for (int i = 1; i < kSumSections; ++i)
-        if (s.part[i].src && blockIdx.x >= s.part[i].first_block) which = i;
+        if (s.part[i].src && block >= s.part[i].first_block) which = i;
     const ColumnSum& p = s.part[which];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t c = (int64_t)(blockIdx.x - p.first_block) * 64 + lane;
+    const int64_t c = (int64_t)(block - p.first_block) * 64 + lane;
     float sum = 0.0f;
     if (c < p.cols) {
 #pragma unroll 8
@@ -138,6 +138,10 @@ __global__ __launch_bounds__(64 * kSumWaves) void column_sums_kernel(ColumnSums 
         for (int w = 1; w < kSumWaves; ++w) sum += shared[w][lane];
         put<T>(p.out, c, p.narrow != 0, sum);
     }
+}
+template <typename T>
+__global__ __launch_bounds__(64 * kSumWaves) void column_sums_kernel(ColumnSums s) {
+    column_sums<T>(s, blockIdx.x);
 }
 
 }  // namespace fmselective

@@ -58,18 +58,23 @@ inline int check_alias(const char* who, std::initializer_list<Range> outs, std::
     return 0;
 }
 
-inline void launch_column_sums(int dtype, std::initializer_list<ColumnSum> parts, hipStream_t stream) {
-    ColumnSums s = {};
+// The sections of one launch, and its blocks
+inline uint32_t column_sections(std::initializer_list<ColumnSum> parts, ColumnSums* s) {
     uint32_t blocks = 0;
     int k = 0;
+    *s = {};
     for (const ColumnSum& p : parts) {
         if (!p.out) continue;
-        s.part[k] = p;
-        s.part[k].first_block = blocks;
+        s->part[k] = p;
+        s->part[k].first_block = blocks;
         blocks += (uint32_t)((p.cols + 63) / 64);
         ++k;
     }
-    if (!blocks) return;
+    return blocks;
+}
+inline void launch_column_sums(int dtype, std::initializer_list<ColumnSum> parts, hipStream_t stream) {
+    ColumnSums s;
+    const uint32_t blocks = column_sections(parts, &s);
     with_dtype(dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
         column_sums_kernel<T><<<blocks, 64 * kSumWaves, 0, stream>>>(s);

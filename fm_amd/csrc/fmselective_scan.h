@@ -654,36 +654,52 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
     }
 }
 
-// The gradients of write and read: the blocks' sums added up in their order and rounded once. A wave a
-// (b, g, n, mark), a float4 a lane, in the order that sum_rows left them.
+// The last sums of a backward call, in one launch. The first blocks take the parameters' gradients (column_sums); the
+// others the gradients of write and read: the partial sums added up in a fixed order and rounded once, `per` waves of
+// a block for one (b, g, n, mark), each every per-th partial sum, a float4 a lane, in the order that the backward
+// kernel left them.
 template <typename T>
-__global__ __launch_bounds__(256) void selective_shared_grads_kernel(const float* __restrict__ part, T* __restrict__ write_grad,
-                                                                     T* __restrict__ read_grad, const int32_t* __restrict__ lengths,
-                                                                     int64_t L, int64_t waves, int32_t N, int32_t G,
-                                                                     int32_t marks, int32_t blocks) {
-    const int lane = threadIdx.x & 63, part_of = lane >> 4, c = lane & 15;
-    const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (wave >= waves) return;
-    const int64_t line = wave / marks;  // (b, g, n)
-    const int32_t mark = (int32_t)(wave - line * marks);
+__global__ __launch_bounds__(64 * kSumWaves) void selective_sums_kernel(ColumnSums columns, uint32_t column_blocks,
+                                                                        const float* __restrict__ part, T* __restrict__ write_grad,
+                                                                        T* __restrict__ read_grad, const int32_t* __restrict__ lengths,
+                                                                        int64_t L, int64_t items, int32_t N, int32_t G,
+                                                                        int32_t marks, int32_t blocks, int32_t per) {
+    if (blockIdx.x < column_blocks) {
+        column_sums<T>(columns, blockIdx.x);
+        return;
+    }
+    __shared__ float4 shared[kSumWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, turn = wave & (per - 1);
+    const int64_t item = ((int64_t)(blockIdx.x - column_blocks) * kSumWaves + wave) / (uint32_t)per;
+    const int64_t line = item / marks;  // (b, g, n)
+    const int32_t mark = (int32_t)(item - line * marks);
     const int64_t bg = line / N;
     const int32_t n = (int32_t)(line - bg * N);
-    const int64_t len = row_length(lengths, bg / G, L);
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int64_t len = item < items ? row_length(lengths, bg / G, L) : 0;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if ((int64_t)mark * kMark < len) {
         const float4* at = reinterpret_cast<const float4*>(part) + (((bg * blocks) * N + n) * marks + mark) * 64 + lane;
         const int64_t step = (int64_t)N * marks * 64;
 #pragma unroll 4
-        for (int32_t i = 0; i < blocks; ++i) {
+        for (int32_t i = turn; i < blocks; i += per) {
             const float4 v = at[i * step];
-            s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
     }
+    shared[wave][lane] = s;
+    __syncthreads();
+    if (turn || item >= items) return;
+    for (int w = 1; w < per; ++w) {
+        const float4 v = shared[wave + w][lane];
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    const float sum[4] = {s.x, s.y, s.z, s.w};
+    const int part_of = lane >> 4, c = lane & 15;
     T* out = (part_of < 2 ? write_grad : read_grad) + line * L;
     const int64_t t0 = (int64_t)mark * kMark + c * kSteps + (part_of & 1) * 4;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        if (t0 + k < L) out[t0 + k] = t0 + k < len ? (T)s[k] : (T)0.0f;
+        if (t0 + k < L) out[t0 + k] = t0 + k < len ? (T)sum[k] : (T)0.0f;
 }
 
 struct Step {

@@ -91,8 +91,8 @@ int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselecti
     }
     float* const pairs = (float*)workspace + b.shared;
     const Scan p = scan_of(*in, 4 * kBackWaves, b.cut, pairs);
-    const int64_t lines = in->B * in->G * in->N, waves = lines * p.marks, blocks = b.blocks * b.cut.segments;
-    if (blocks > INT32_MAX || waves > (int64_t)INT32_MAX * 4)
+    const int64_t lines = in->B * in->G * in->N, items = lines * p.marks, blocks = b.blocks * b.cut.segments;
+    if (blocks > INT32_MAX || items > INT32_MAX - (1 << 24))
         return fail(FMSCAN_E_SHAPE, "%s: B * D or B * G * N * L is too large for one launch", who);
     float* part = (float*)workspace;
     ScanGrads g = {};
@@ -115,17 +115,20 @@ int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselecti
         const hipStream_t st = (hipStream_t)stream;
         if (b.cut.segments > 1 && (rc = launch_backward<T, true>(who, p, g, blocks, st))) return;
         if ((rc = launch_backward<T, false>(who, p, g, blocks, st))) return;
-        fmselective::selective_shared_grads_kernel<T><<<(unsigned)((waves + 3) / 4), 256, 0, (hipStream_t)stream>>>(
-            part, (T*)o.write, (T*)o.read, in->lengths, in->L, waves, p.N, p.G, p.marks, p.blocks_per_group);
-        rc = launched("selective scan (gradients of write and read)");
+        fmselective::ColumnSums columns;
+        const uint32_t column_blocks = column_sections(
+            {{g.A_part, o.A, in->B * b.cut.segments, in->D * in->N, 0, 0},
+             {g.skip_part, o.skip, in->B * b.cut.segments, in->D, (in->flags & FMSELECTIVE_NARROW_SKIP) != 0, 0},
+             {g.bias_part, o.delta_bias, in->B * b.cut.segments, in->D, (in->flags & FMSELECTIVE_NARROW_BIAS) != 0, 0}}, &columns);
+        constexpr int W = fmselective::kSumWaves;
+        int per = 1;  // waves that share a sum: at least four terms each
+        while (per < W && p.blocks_per_group >= 8 * per) per *= 2;
+        fmselective::selective_sums_kernel<T><<<(unsigned)(column_blocks + (items * per + W - 1) / W), 64 * W, 0, st>>>(
+            columns, column_blocks, part, (T*)o.write, (T*)o.read, in->lengths, in->L, items, p.N, p.G, p.marks,
+            p.blocks_per_group, per);
+        rc = launched("selective scan (sums of gradients)");
     });
-    if (rc) return rc;
-    launch_column_sums(in->dtype,
-                       {{g.A_part, o.A, in->B * b.cut.segments, in->D * in->N, 0, 0},
-                        {g.skip_part, o.skip, in->B * b.cut.segments, in->D, (in->flags & FMSELECTIVE_NARROW_SKIP) != 0, 0},
-                        {g.bias_part, o.delta_bias, in->B * b.cut.segments, in->D, (in->flags & FMSELECTIVE_NARROW_BIAS) != 0, 0}},
-                       (hipStream_t)stream);
-    return launched("selective scan (sums of the parameters' gradients)");
+    return rc;
 }
 
 }  // extern "C"

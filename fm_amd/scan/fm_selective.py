@@ -159,7 +159,7 @@ def _conv_backward(inputs, weight, bias, initial_state, lengths, silu, out_grad,
         if want_state:
             d_state = torch.zeros((B, D, W - 1), dtype=inputs.dtype, device=dev) if final_grad is None else final_grad
         return (torch.zeros_like(inputs), torch.zeros_like(weight), None if bias is None else torch.zeros_like(bias), d_state)
-    d_inputs = torch.empty((B, D, L), dtype=inputs.dtype, device=dev)
+    d_inputs = torch.empty_like(inputs, memory_format=torch.contiguous_format)
     d_weight = torch.empty_like(weight)
     d_bias = None if bias is None else torch.empty_like(bias)
     d_state = torch.empty((B, D, W - 1), dtype=inputs.dtype, device=dev) if want_state else None
@@ -344,8 +344,8 @@ def _scan_backward(inputs, softplus, marks, out_grad, final_grad, want_state):
             d_state = torch.zeros((B, D, N), dtype=torch.float32, device=dev) if final_grad is None else final_grad
         zeros = [None if t is None else torch.zeros_like(t) for t in (tokens, delta, A, write, read, skip, gate, delta_bias)]
         return (*zeros, d_state)
-    new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
-    grads = [new(t) for t in (tokens, delta, A, write, read, skip, gate, delta_bias)]
+    grads = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
+             for t in (tokens, delta, A, write, read, skip, gate, delta_bias)]
     d_tokens, d_delta, d_A, d_write, d_read, d_skip, d_gate, d_bias = grads
     d_state = torch.empty((B, D, N), dtype=torch.float32, device=dev) if want_state else None
     need = _raw.fmselective_scan_workspace_bytes(*sizes, 1)
