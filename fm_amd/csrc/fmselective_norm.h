@@ -161,7 +161,8 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_forward_kernel(con
 }
 
 // dr = dresidual + (dy w - x mean(dy w x)) / rms with x = r / rms;  dweight = sum over the rows of dy x.
-// A block (a wave, for short rows) takes every gridDim-th row and keeps its part of the weight's gradient in registers.
+// A block (a wave, for short rows) takes every slots-th row and keeps its part of the weight's gradient in registers;
+// each block leaves one part.
 template <typename T, int TPR, int CH>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_backward_kernel(const T* __restrict__ out_grad,
                                                                               const T* __restrict__ residual_grad,
@@ -220,8 +221,27 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_backward_kernel(co
             store_values<T, E>(grad + row * D, ((int64_t)j * TPR + i) * E, D, g);
         }
     }
+    float* part = weight_part + (int64_t)blockIdx.x * D;
+    if constexpr (RPB > 1) {  // the block's waves hold parts of the same columns
+        __shared__ float held[RPB - 1][CH][E][64];
+        const int wave = threadIdx.x >> 6;
+        if (wave) {
 #pragma unroll
-    for (int j = 0; j < CH; ++j) store_values<float, E>(weight_part + slot * D, ((int64_t)j * TPR + i) * E, D, dw[j]);
+            for (int j = 0; j < CH; ++j)
+#pragma unroll
+                for (int k = 0; k < E; ++k) held[wave - 1][j][k][i] = dw[j][k];
+        }
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int w = 0; w < RPB - 1; ++w)
+#pragma unroll
+            for (int j = 0; j < CH; ++j)
+#pragma unroll
+                for (int k = 0; k < E; ++k) dw[j][k] += held[w][j][k][i];
+    }
+#pragma unroll
+    for (int j = 0; j < CH; ++j) store_values<float, E>(part, ((int64_t)j * TPR + i) * E, D, dw[j]);
 }
 
 }  // namespace fmselective

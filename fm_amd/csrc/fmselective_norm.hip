@@ -32,12 +32,14 @@ void with_row_shape(int64_t D, int dtype, F&& f) {
     else f(IntTag<1024>{}, IntTag<4>{});  // FMSELECTIVE_MAX_NORM float32 values are 4096 chunks
 }
 
-// Rows that work side by side in the backward call, each slot with its part of the weight's gradient: enough for
-// the memory's latency, few enough that the parts are small beside the streams.
-constexpr int64_t kNormSlots = 512;
-int64_t backward_slots(int64_t rows) {
-    int64_t n = (rows + 7) / 8;
-    return n > kNormSlots ? kNormSlots : n;
+// Blocks of the backward call, each with its part of the weight's gradient: all the rows' where there are few, else as
+// many as keep the memory busy and leave the parts small beside the streams.
+#ifndef FMSELECTIVE_NORM_BLOCKS
+#define FMSELECTIVE_NORM_BLOCKS 512
+#endif
+int64_t backward_blocks(int64_t rows, int rows_per_block) {
+    const int64_t n = (rows + rows_per_block - 1) / rows_per_block;
+    return n > FMSELECTIVE_NORM_BLOCKS ? FMSELECTIVE_NORM_BLOCKS : n;
 }
 
 }  // namespace
@@ -77,8 +79,7 @@ int fmselective_norm_forward(const void* inputs, const void* residual, const voi
 
 size_t fmselective_norm_workspace_bytes(int64_t rows, int64_t D, int dtype) {
     if (check_rows("fmselective_norm_workspace_bytes", rows, D, dtype)) return 0;
-    // (short rows go four to a block: whole blocks of four slots)
-    return (size_t)((backward_slots(rows) + 3) / 4 * 4) * D * sizeof(float);
+    return (size_t)backward_blocks(rows, 1) * D * sizeof(float);
 }
 
 int fmselective_norm_backward(const void* out_grad, const void* residual_grad, const void* stream_in, const void* weight,
@@ -100,20 +101,19 @@ int fmselective_norm_backward(const void* out_grad, const void* residual_grad, c
                              {{"out_grad", out_grad, rows * D * es}, {"residual_grad", residual_grad, rows * D * es},
                               {"the stream", stream_in, rows * D * es}, {"weight", weight, D * ws}, {"inv_rms", inv_rms, rows * 4}}))
         return rc;
-    int64_t slots = backward_slots(rows);
+    int64_t blocks = 0;
     with_dtype(dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
         with_row_shape(D, dtype, [&](auto pt, auto ct) {
             constexpr int TPR = decltype(pt)::value, CH = decltype(ct)::value, RPB = TPR == 64 ? 4 : 1;
-            const int64_t blocks = (slots + RPB - 1) / RPB;
-            slots = blocks * RPB;
+            blocks = backward_blocks(rows, RPB);
             fmselective::norm_backward_kernel<T, TPR, CH><<<(unsigned)blocks, TPR == 64 ? 256 : TPR, 0, (hipStream_t)stream>>>(
                 (const T*)out_grad, (const T*)residual_grad, (const T*)stream_in, weight, inv_rms, (T*)grad, (float*)workspace,
                 rows, (int32_t)D, flags);
         });
     });
     if (int rc = launched("norm (backward)")) return rc;
-    launch_column_sums(dtype, {{(const float*)workspace, weight_grad, slots, D, (flags & FMSELECTIVE_NARROW_WEIGHT) != 0, 0}},
+    launch_column_sums(dtype, {{(const float*)workspace, weight_grad, blocks, D, (flags & FMSELECTIVE_NARROW_WEIGHT) != 0, 0}},
                        (hipStream_t)stream);
     return launched("norm (the weight's gradient)");
 }
