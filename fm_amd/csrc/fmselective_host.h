@@ -20,9 +20,9 @@ inline int check_sizes(const char* who, int64_t B, int64_t D, int64_t L, int dty
                     (long long)D, (long long)L);
     if (dtype != FMSCAN_DTYPE_F32 && dtype != FMSCAN_DTYPE_F16 && dtype != FMSCAN_DTYPE_BF16)
         return fail(FMSCAN_E_DTYPE, "%s: dtype %d is not float32 (0), float16 (1) or bfloat16 (2)", who, dtype);
-    if (B > INT32_MAX || D > INT32_MAX || (__int128)B * D > (__int128)INT32_MAX || L > (int64_t)INT32_MAX - 4096 ||
-        (__int128)B * D * L > ((__int128)1 << 40))
-        return fail(FMSCAN_E_SHAPE, "%s: B * D and L must fit 31 bits, B * D * L 40 bits", who);
+    // (a kernel's last block may reach beyond D and L: their 32-bit indexes have room for that)
+    if (D > (1 << 30) || (__int128)B * D > (__int128)INT32_MAX || L > (1 << 30) || (__int128)B * D * L > ((__int128)1 << 40))
+        return fail(FMSCAN_E_SHAPE, "%s: D and L must be at most 2^30, B * D below 2^31 and B * D * L at most 2^40", who);
     return 0;
 }
 inline int check_flags(const char* who, unsigned flags, unsigned known) {

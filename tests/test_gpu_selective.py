@@ -1,4 +1,6 @@
 """The selective layer's operators on the GPU against plain implementations in float64 (selective_reference.py)."""
+import math
+
 import pytest
 import torch
 
@@ -664,3 +666,96 @@ def test_nothing_to_do(m, nm):
     assert y.shape == (0, 8)
     q, s, _ = nm.fm_norm_quantized(z(2, 0, 8), z(8))
     assert q.shape == (2, 0, 8) and s.shape == (2, 0)
+
+
+def test_broadcast_inputs_get_summed_gradients(m):
+    """write and read shared by the batch, one gate for all channels: views of stride zero, whose gradients are sums."""
+    g = gen(51)
+    B, D, L, N = 3, 10, 150, 4
+    a, dy, *_ = scan_case((B, D, L, N, 1), F32, 0)
+    shared = {"write": rand(g, 1, 1, N, L), "read": rand(g, 1, 1, N, L), "gate": rand(g, B, 1, L)}
+    wide = {"write": (B, 1, N, L), "read": (B, 1, N, L), "gate": (B, D, L)}
+    for t in shared.values():
+        t.requires_grad_()
+    a.update({k: t.expand(wide[k]) for k, t in shared.items()})
+    y = m.fm_selective_scan(**a)
+    grads = torch.autograd.grad(y, list(shared.values()), dy)
+    ref = scan_reference(a, True, dy)
+    R.close(y, *ref["y"], 44, "y")
+    for (k, t), got in zip(shared.items(), grads):
+        axis = 1 if k == "gate" else 0
+        v, mag = (x.sum(axis, keepdim=True) for x in ref[GRADS[k]])
+        R.close(got, v, mag, 80 + 2 * N + 40 + D, k)  # (the sum adds at most ten roundings)
+
+
+def test_offsets_beyond_32_bits(m, nm):
+    """Strides, pools and outputs whose elements lie more than 2^31 apart."""
+    g = gen(52)
+    far = (1 << 31) + 24
+    B, D, L, N = 2, 3, 40, 4
+    a, *_ = scan_case((B, D, L, N, 1), BF16, 0)
+    buf = torch.zeros(far + (1 << 16), dtype=BF16, device=DEV)
+    def apart(t, at):  # batch element 1 lies `far` elements behind batch element 0
+        shape = t.shape
+        strides = [far] + [math.prod(shape[i + 1:]) for i in range(1, t.dim())]
+        view = buf.as_strided(shape, strides, at)
+        view.copy_(t)
+        return view
+    near = m.fm_selective_scan(**a)
+    at, moved = 0, dict(a)
+    for k in ("tokens", "delta", "gate", "write", "read"):
+        moved[k] = apart(a[k], at)
+        at += 4096
+    assert torch.equal(m.fm_selective_scan(**moved), near)
+    w = rand(g, D, 4, dtype=BF16)
+    assert torch.equal(m.fm_conv(moved["tokens"], w), m.fm_conv(a["tokens"], w))
+    del buf, moved
+    # a pool of states of more than 2^31 values: the named slots alone are touched
+    D, N = 4096, 16
+    S = (1 << 31) // (D * N) + 3
+    pool = torch.zeros(S, D, N, device=DEV)
+    a, *_ = scan_case((2, D, 1, N, 1), BF16, 0)
+    one = {k: a[k][..., 0].contiguous() for k in ("tokens", "delta", "gate", "write", "read")}
+    slots = torch.tensor([S - 1, 1], device=DEV)
+    small = torch.zeros(2, D, N, device=DEV)
+    y = m.fm_selective_step(state=pool, A=a["A"], slots=slots, **one)
+    assert torch.equal(y, m.fm_selective_step(state=small, A=a["A"], **one))
+    assert torch.equal(pool[slots], small)
+    pool[slots] = 0
+    assert not pool.any()
+    del pool
+    # outputs of more than 2^31 values
+    D, L = 4099, 1 << 19
+    x = torch.zeros(1, D, L, dtype=BF16, device=DEV)
+    x[0, -1] = rand(g, L, dtype=BF16)
+    w = rand(g, D, 4, dtype=BF16)
+    y = m.fm_conv(x, w)
+    assert torch.equal(y[:, -1:], m.fm_conv(x[:, -1:].contiguous(), w[-1:].contiguous())) and not y[0, -2].any()
+    rows = x.view(-1, 4096)
+    y, _ = nm.fm_norm(rows, w.new_ones(4096))
+    assert torch.equal(y[-128:], nm.fm_norm(rows[-128:].contiguous(), w.new_ones(4096))[0])
+
+
+def test_calls_from_two_threads(m):
+    """Two threads, each on a stream of its own: what each gets is what it gets alone."""
+    import threading
+
+    cases = [scan_case((2, 20, 300, 8, 1), BF16, 2, seed=s)[0] for s in (1, 2)]
+    w = [rand(gen(s), 20, 4, dtype=BF16) for s in (1, 2)]
+    work = lambda i: m.fm_selective_scan(**{**cases[i], "tokens": m.fm_conv(cases[i]["tokens"], w[i])}, return_state=True)  # noqa: E731
+    want = [work(i) for i in (0, 1)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = work(i)
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    assert not bad

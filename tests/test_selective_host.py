@@ -45,7 +45,8 @@ def test_conv_rejects(lib):
 
     assert fwd(x=None) == code("NULL") and fwd(w=None) == code("NULL") and fwd(out=None) == code("NULL")
     assert fwd(W=1) == code("SHAPE") and fwd(W=5) == code("SHAPE") and fwd(L=0) == code("SHAPE") and fwd(B=0) == code("SHAPE")
-    assert fwd(B=1 << 20, D=1 << 20) == code("SHAPE") and fwd(L=1 << 31) == code("SHAPE") and fwd(sb=-1) == code("SHAPE")
+    assert fwd(B=1 << 20, D=1 << 20) == code("SHAPE") and fwd(L=(1 << 30) + 1) == code("SHAPE") and fwd(sb=-1) == code("SHAPE")
+    assert fwd(B=1, D=(1 << 30) + 1) == code("SHAPE") and fwd(B=1 << 15, D=1 << 15, L=1 << 11) == code("SHAPE")
     assert fwd(dtype=3) == code("DTYPE") and fwd(flags=1) == code("FLAGS") and fwd(flags=0x100) == code("FLAGS")
     assert fwd(out=P + 16) == code("ALIAS") and fwd(f=3 * P + 8) == code("ALIAS") and fwd(s=4 * P, f=4 * P) == code("ALIAS")
     assert b"overlaps" in lib.fmscan_last_error()
