@@ -33,13 +33,12 @@ void with_row_shape(int64_t D, int dtype, F&& f) {
 }
 
 // Blocks of the backward call, each with its part of the weight's gradient: all the rows' where there are few, else as
-// many as keep the memory busy and leave the parts small beside the streams.
-#ifndef FMSELECTIVE_NORM_BLOCKS
-#define FMSELECTIVE_NORM_BLOCKS 512
-#endif
+// many as keep the memory busy and leave the parts small beside the streams. Measured with 512, 768, 1024 blocks (bf16,
+// us, the parts' sum included): (8192, 4096) 54, 56, 64; (16384, 1024) 30, 30, 36; (9208, 1297) 61, 51, 47.
+constexpr int64_t kNormBlocks = 512;
 int64_t backward_blocks(int64_t rows, int rows_per_block) {
     const int64_t n = (rows + rows_per_block - 1) / rows_per_block;
-    return n > FMSELECTIVE_NORM_BLOCKS ? FMSELECTIVE_NORM_BLOCKS : n;
+    return n > kNormBlocks ? kNormBlocks : n;
 }
 
 }  // namespace

@@ -6,20 +6,20 @@ using fmselective::Scan;
 
 namespace {
 
-// Lanes a channel: 16, so that a wave works on 4 channels, or all 64 where that leaves too few waves; and where
-// that is too few as well, the rows are cut.
-#ifndef FMSELECTIVE_FEW_WAVES
-#define FMSELECTIVE_FEW_WAVES 2048
-#endif
-#ifndef FMSELECTIVE_CUT_BELOW
-#define FMSELECTIVE_CUT_BELOW 1024
-#endif
-#ifndef FMSELECTIVE_CUT_WANT
-#define FMSELECTIVE_CUT_WANT 2048
-#endif
-#ifndef FMSELECTIVE_WAVES64
-#define FMSELECTIVE_WAVES64 8
-#endif
+// Lanes a channel: 16, so that a wave works on 4 channels, or all 64, so that four times as many waves work on tiles of
+// four times the length. Measured for N = 16, bf16, on tiles of one wave: with up to two waves a SIMD a tile takes 5 to
+// 7 us of 16 lanes (128 steps of four channels) and 7 to 8 us of 64 (512 of one), the instructions' latency; with more
+// it is their number that counts, 3.1 and 3.5 us for each of a SIMD's waves. The faster of the two by that is taken:
+// (7, 1024, 515) 57 -> 40 us with 16 lanes, (1, 4096, 16384) 680 -> 440 with 64, (1, 4096, 500) 26 -> 20.
+// Where 64 lanes leave less than two waves a SIMD the rows are cut, for four: (1, 1024, 16384) 225 -> 179 us,
+// (1, 512, 16384) 112 -> 95 (against a cut for two).
+constexpr int64_t kSimds = 1024;
+constexpr int64_t kCutBelow = 2 * kSimds, kCutWant = 4 * kSimds;
+int64_t modelled_time(int64_t tiles, int64_t waves, int64_t latency, int64_t each) {  // in units of 0.1 us / 1024
+    const int64_t busy = each * waves;
+    return tiles * (busy > latency * kSimds ? busy : latency * kSimds);
+}
+
 // A single token's call: blocks of 64 channels from which on a block takes 256 instead
 constexpr int64_t kManyStepBlocks = 4096;
 
@@ -30,10 +30,11 @@ struct ForwardPlan {
 };
 ForwardPlan plan_forward(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) {
     ForwardPlan f;
-    const int64_t waves = B * G * ((D / G + 3) / 4);
-    f.lanes = waves >= FMSELECTIVE_FEW_WAVES || L <= 128 ? 16 : 64;
-    const int64_t have = f.lanes == 16 ? waves : B * D, tile = f.lanes * fmselective::kSteps;
-    f.cut = cut_of((L + tile - 1) / tile, have, have < FMSELECTIVE_CUT_BELOW ? FMSELECTIVE_CUT_WANT : have);
+    const int64_t waves16 = B * G * ((D / G + 3) / 4), waves64 = B * D;
+    const int64_t tiles16 = (L + 127) / 128, tiles64 = (L + 511) / 512;
+    f.lanes = modelled_time(tiles16, waves16, 65, 31) <= modelled_time(tiles64, waves64, 75, 35) ? 16 : 64;
+    // (16 lanes are only taken where the rows are short or many: not cut)
+    f.cut = f.lanes == 16 ? Cut{1, (int32_t)tiles16} : cut_of(tiles64, waves64, waves64 < kCutBelow ? kCutWant : waves64);
     f.bytes = f.cut.segments > 1 ? (size_t)(f.cut.segments - 1) * B * D * N * sizeof(float2) : 0;
     return f;
 }
@@ -98,7 +99,7 @@ int fmselective_scan_forward(const fmselective_scan_inputs* in, void* out, float
         using T = typename decltype(tt)::type;
         constexpr int W = fmselective::kScanWaves;
         rc = f.lanes == 16 ? launch_forward<T, 16, W>(who, *in, f.cut, out, final_state, marks, workspace, (hipStream_t)stream)
-                           : launch_forward<T, 64, FMSELECTIVE_WAVES64>(who, *in, f.cut, out, final_state, marks, workspace, (hipStream_t)stream);
+                           : launch_forward<T, 64, 8>(who, *in, f.cut, out, final_state, marks, workspace, (hipStream_t)stream);
     });
     return rc;
 }

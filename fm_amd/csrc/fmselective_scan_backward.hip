@@ -9,13 +9,10 @@ namespace {
 
 constexpr int kBackWaves = fmselective::kScanWaves;
 
-// The rows are cut where they leave too few waves.
-#ifndef FMSELECTIVE_BACK_CUT_BELOW
-#define FMSELECTIVE_BACK_CUT_BELOW 1024
-#endif
-#ifndef FMSELECTIVE_BACK_CUT_WANT
-#define FMSELECTIVE_BACK_CUT_WANT 2048
-#endif
+// The rows are cut where they leave less than a wave a SIMD, for two. Measured (bf16, N = 16, us): (1, 2048, 2048), 512
+// waves, 144 with one wave a SIMD, 102 with two, 104 with four; (1, 1024, 8192) 285, 193, 194; at (1, 4096, 2048),
+// 1024 waves, the cut gains nothing (203, 202).
+constexpr int64_t kBackCutBelow = 1024, kBackCutWant = 2048;
 struct BackPlan {
     Cut cut;
     int64_t blocks, shared, states, rows, pairs;  // blocks; floats of the partial sums and of the pairs
@@ -26,7 +23,7 @@ BackPlan plan_backward(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) {
     BackPlan b;
     b.blocks = B * G * ((per_group + 4 * kBackWaves - 1) / (4 * kBackWaves));
     const int64_t waves = b.blocks * kBackWaves;
-    b.cut = cut_of(marks, waves, waves < FMSELECTIVE_BACK_CUT_BELOW ? FMSELECTIVE_BACK_CUT_WANT : waves);
+    b.cut = cut_of(marks, waves, waves < kBackCutBelow ? kBackCutWant : waves);
     b.shared = b.blocks * N * marks * 256;
     b.pairs = b.cut.segments > 1 ? 2 * b.cut.segments * B * D * N : 0;
     b.states = b.cut.segments * B * D * N;
