@@ -107,13 +107,31 @@ template <typename T>
 struct Raw {
     u32x4 v[kSteps / Elem<T>::E];
 };
+// (whole, the same in all lanes: all their steps count, and the loads need no condition)
 template <typename T>
-__device__ __forceinline__ Raw<T> load_raw(const T* __restrict__ row, int64_t t0, int64_t len) {
+__device__ __forceinline__ Raw<T> load_raw(const T* __restrict__ row, int64_t t0, int64_t len, bool whole) {
     Raw<T> r;
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < kSteps / Elem<T>::E; ++i)
-        r.v[i] = fmscan::load_chunk<T, false, false>(row, t0 + i * Elem<T>::E, len, 0u);
+        for (int i = 0; i < kSteps / Elem<T>::E; ++i) r.v[i] = fmscan::load16<T, false, false>(row + t0 + i * Elem<T>::E);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSteps / Elem<T>::E; ++i)
+            r.v[i] = fmscan::load_chunk<T, false, false>(row, t0 + i * Elem<T>::E, len, 0u);
+    }
     return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_steps(T* __restrict__ row, int64_t t0, int64_t L, bool whole, const float (&f)[kSteps]) {
+    constexpr int E = Elem<T>::E;
+    if (!whole) return store_values<T, kSteps>(row, t0, L, f);
+#pragma unroll
+    for (int i = 0; i < kSteps / E; ++i) {
+        float part[E];
+#pragma unroll
+        for (int k = 0; k < E; ++k) part[k] = f[i * E + k];
+        fmscan::store16<T, false>(row + t0 + i * E, Elem<T>::pack(part));
+    }
 }
 template <typename T>
 __device__ __forceinline__ void widen_raw(const Raw<T>& r, float (&f)[kSteps]) {
@@ -149,11 +167,12 @@ struct TileLoader {
     Raw<T> raw[kEach];
     __device__ __forceinline__ void load(const T* write, int64_t write_n, const T* read, int64_t read_n, int n0, int N,
                                          int64_t tile_t0, int64_t len) {
+        const bool whole = n0 + NC <= N && tile_t0 + LPC * kSteps <= len;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
             const int i = threadIdx.x + j * 64 * WAVES, which = i / kChunks, n = n0 + (i / LPC) % NC, c = i % LPC;
             const T* rows = which ? read + n * read_n : write + n * write_n;
-            raw[j] = load_raw<T>(rows, tile_t0 + c * kSteps, n < N ? len : 0);
+            raw[j] = load_raw<T>(rows, tile_t0 + c * kSteps, n < N ? len : 0, whole);
         }
     }
     __device__ __forceinline__ void put(SharedTile<LPC, NC>& t) const {
@@ -236,6 +255,7 @@ __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T
     const int32_t d = (int32_t)g * p.per_group + (valid ? local : p.per_group - 1);
     const int64_t row = (int64_t)b * p.D + d;
     const int64_t len = row_length(p.lengths, b, p.L), mine = valid ? len : 0;  // (no steps for a channel beyond the group)
+    const bool all_valid = __all(valid);
     const T* u_row = (const T*)p.tokens + b * p.tokens_b + d * p.tokens_d;
     const T* delta_row = (const T*)p.delta + b * p.delta_b + d * p.delta_d;
     const T* gate_row = p.gate ? (const T*)p.gate + b * p.gate_b + d * p.gate_d : nullptr;
@@ -270,9 +290,10 @@ __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T
     };
     auto fetch_rows = [&](int32_t tile) {
         const int64_t t0 = (int64_t)tile * kTile + c * kSteps;
-        next_u = load_raw<T>(u_row, t0, mine);
-        next_delta = load_raw<T>(delta_row, t0, mine);
-        if (!ENDS && gate_row) next_gate = load_raw<T>(gate_row, t0, mine);
+        const bool whole = all_valid && (int64_t)(tile + 1) * kTile <= len;
+        next_u = load_raw<T>(u_row, t0, mine, whole);
+        next_delta = load_raw<T>(delta_row, t0, mine, whole);
+        if (!ENDS && gate_row) next_gate = load_raw<T>(gate_row, t0, mine, whole);
     };
     if (total) {
         fetch_shared(first_tile, 0);
@@ -355,7 +376,7 @@ __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) y[k] = k < left ? y[k] : 0.0f;
         }
-        if (valid) store_values<T, kSteps>(out + row * p.L, t0, p.L, y);
+        if (valid) store_steps<T>(out + row * p.L, t0, p.L, !ragged, y);
     }
     if constexpr (ENDS) {
         // (the total's decay in one exponential of the summed steps, as within a tile)
@@ -426,6 +447,7 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
     const int32_t d = (int32_t)g * p.per_group + (valid ? local : p.per_group - 1);
     const int64_t row = (int64_t)b * p.D + d;
     const int64_t len = row_length(p.lengths, b, p.L), mine = valid ? len : 0;
+    const bool all_valid = __all(valid);
     const float skip = p.skip ? param<T>(p.skip, d, p.flags & FMSELECTIVE_NARROW_SKIP) : 0.0f;
     const float bias = p.delta_bias ? param<T>(p.delta_bias, d, p.flags & FMSELECTIVE_NARROW_BIAS) : 0.0f;
     float skip_sum = 0.0f, bias_sum = 0.0f, all_dt = 0.0f;
@@ -470,11 +492,12 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
         const bool ragged = (int64_t)(tile + 1) * kTile > len;
         const int left = ragged ? steps_left(mine, t0) : kSteps;
         float dt[kSteps], dtu[kSteps], gy[kSteps], sum_w[kSteps], sum_a[kSteps], y[kSteps], total_dt = 0.0f;
+        const bool whole = all_valid && !ragged;
+        const Raw<T> raw_d = load_raw<T>(delta_row, t0, mine, whole), raw_g = load_raw<T>(dy_row, t0, mine, whole);
+        Raw<T> raw_u = {}, raw_z = {};
         {
-            const Raw<T> raw_d = load_raw<T>(delta_row, t0, mine), raw_g = load_raw<T>(dy_row, t0, mine);
-            Raw<T> raw_u = {}, raw_z = {};
-            if (!ENDS) raw_u = load_raw<T>(u_row, t0, mine);
-            if (gate_row) raw_z = load_raw<T>(gate_row, t0, mine);
+            if (!ENDS) raw_u = load_raw<T>(u_row, t0, mine, whole);
+            if (gate_row) raw_z = load_raw<T>(gate_row, t0, mine, whole);
             if (!ENDS)
                 for (int n = c; n < p.N; n += LPC) held[n].w = valid ? o.marks[(row * p.marks + tile) * p.N + n] : 0.0f;
             float u[kSteps], z[kSteps];
@@ -587,8 +610,8 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
         }
         if (ENDS) continue;
         float u[kSteps], dd[kSteps], x[kSteps], z[kSteps];
-        load_values<T, kSteps>(u_row, t0, mine, u);
-        load_values<T, kSteps>(delta_row, t0, mine, x);
+        widen_raw(raw_u, u);
+        widen_raw(raw_d, x);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
             dd[k] = __builtin_fmaf(u[k], sum_w[k], kLn2 * sum_a[k]);
@@ -609,19 +632,19 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
             skip_sum = __builtin_fmaf(gy[k], u[k], skip_sum);
         }
         if (valid) {
-            store_values<T, kSteps>((T*)o.tokens + row * p.L, t0, p.L, x);
-            store_values<T, kSteps>((T*)o.delta + row * p.L, t0, p.L, dd);
+            store_steps<T>((T*)o.tokens + row * p.L, t0, p.L, !ragged, x);
+            store_steps<T>((T*)o.delta + row * p.L, t0, p.L, !ragged, dd);
         }
         if (gate_row) {
-            load_values<T, kSteps>(dy_row, t0, mine, dd);
-            load_values<T, kSteps>(gate_row, t0, mine, z);
+            widen_raw(raw_g, dd);
+            widen_raw(raw_z, z);
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) dd[k] *= y[k] * silu_slope(z[k], sigmoid(z[k]));
             if (ragged) {
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) dd[k] = k < left ? dd[k] : 0.0f;
             }
-            if (valid) store_values<T, kSteps>((T*)o.gate + row * p.L, t0, p.L, dd);
+            if (valid) store_steps<T>((T*)o.gate + row * p.L, t0, p.L, !ragged, dd);
         }
     }
     if constexpr (ENDS) {
