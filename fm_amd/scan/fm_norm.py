@@ -11,11 +11,10 @@ float32, float16 and bfloat16; statistics and gradient sums in float32. The kern
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .fm_scan import _ptr, _raw, _require
-from .fm_selective import _call, _dense, _gpu, _parameter, _tracked, _type_of
+from .fm_selective import _call, _dense, _gpu, _once, _parameter, _tracked, _type_of
 
 __all__ = ["fm_norm", "fm_norm_quantized", "FM_Norm"]
 
@@ -40,8 +39,8 @@ def _check(inputs, weight, residual, eps):
 
 
 def _forward(inputs, weight, residual, eps, save=False, quantized=False):
-    """(out, residual_out or None, inv_rms or None, scales or None)"""
-    rows, D, code, flags = _check(inputs, weight, residual, eps)
+    """(out, residual_out or None, inv_rms or None, scales or None, the checked sizes)"""
+    sizes = rows, D, code, flags = _check(inputs, weight, residual, eps)
     dev, shape = inputs.device, inputs.shape
     out = torch.empty(shape, dtype=torch.float8_e4m3fn if quantized else inputs.dtype, device=dev)
     stream_out = None if residual is None else torch.empty(shape, dtype=inputs.dtype, device=dev)
@@ -52,7 +51,7 @@ def _forward(inputs, weight, residual, eps, save=False, quantized=False):
               out.data_ptr(), _ptr(scales), _ptr(inv_rms), rows, D, code, flags, float(eps))
     elif quantized:
         scales.zero_()
-    return out, stream_out, inv_rms, scales
+    return out, stream_out, inv_rms, scales, sizes
 
 
 class FM_Norm(torch.autograd.Function):
@@ -61,33 +60,36 @@ class FM_Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, inputs, weight, residual=None, eps=1e-6):
         save = any(ctx.needs_input_grad)
-        out, stream_out, inv_rms, _ = _forward(inputs, weight, residual, eps, save=save)
+        out, stream_out, inv_rms, _, ctx.sizes = _forward(inputs, weight, residual, eps, save=save)
         if save:
             ctx.save_for_backward(inputs if residual is None else stream_out, weight, inv_rms)
         ctx.set_materialize_grads(False)
         return out, stream_out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, out_grad, residual_grad):
-        stream_in, weight, inv_rms = ctx.saved_tensors
-        if out_grad is None and residual_grad is None:
-            return None, None, None, None
-        if out_grad is None:  # nothing goes through the norm
-            return residual_grad, torch.zeros_like(weight), residual_grad, None
-        rows, D, code, flags = _check(stream_in, weight, None, 0.0)
-        dev = stream_in.device
-        grad, d_weight = torch.empty_like(stream_in), torch.empty_like(weight)
-        if not rows:
-            return grad, d_weight.zero_(), grad, None
-        out_grad = out_grad.contiguous()
-        residual_grad = None if residual_grad is None else residual_grad.contiguous()
-        need = _raw.fmselective_norm_workspace_bytes(rows, D, code)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        _call(dev, _raw.fmselective_norm_backward, out_grad.data_ptr(), _ptr(residual_grad), stream_in.data_ptr(),
-              weight.data_ptr(), inv_rms.data_ptr(), grad.data_ptr(), d_weight.data_ptr(), rows, D, code, flags,
-              workspace.data_ptr(), need)
-        return grad, d_weight, grad if ctx.needs_input_grad[2] else None, None
+        return _once(_norm_gradients, ctx, out_grad, residual_grad)
+
+
+def _norm_gradients(ctx, out_grad, residual_grad):
+    if out_grad is None and residual_grad is None:
+        return None, None, None, None
+    stream_in, weight, inv_rms = ctx.saved_tensors
+    if out_grad is None:  # nothing goes through the norm
+        return residual_grad, torch.zeros_like(weight), residual_grad, None
+    rows, D, code, flags = ctx.sizes
+    dev = stream_in.device
+    grad, d_weight = torch.empty_like(stream_in), torch.empty_like(weight)
+    if not rows:
+        return grad, d_weight.zero_(), grad, None
+    out_grad = out_grad.contiguous()
+    residual_grad = None if residual_grad is None else residual_grad.contiguous()
+    need = _raw.fmselective_norm_workspace_bytes(rows, D, code)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    _call(dev, _raw.fmselective_norm_backward, out_grad.data_ptr(), _ptr(residual_grad), stream_in.data_ptr(),
+          weight.data_ptr(), inv_rms.data_ptr(), grad.data_ptr(), d_weight.data_ptr(), rows, D, code, flags,
+          workspace.data_ptr(), need)
+    return grad, d_weight, grad if ctx.needs_input_grad[2] else None, None
 
 
 def fm_norm(inputs, weight, residual=None, eps=1e-6):
@@ -105,7 +107,7 @@ def fm_norm(inputs, weight, residual=None, eps=1e-6):
     if _tracked(inputs, weight, residual):
         out, stream_out = FM_Norm.apply(inputs, weight, residual, eps)
     else:
-        out, stream_out, _, _ = _forward(inputs, weight, residual, eps)
+        out, stream_out, _, _, _ = _forward(inputs, weight, residual, eps)
     return out, (inputs if residual is None else stream_out)
 
 
@@ -116,5 +118,5 @@ def fm_norm_quantized(inputs, weight, residual=None, eps=1e-6):
     max |out| / 448 of each row, values are rounded to nearest even. A row of zeros, or of values below 2^-100, has scale
     0; a row with a NaN among its outputs has a NaN scale.
     """
-    out, stream_out, _, scales = _forward(inputs, weight, residual, eps, quantized=True)
+    out, stream_out, _, scales, _ = _forward(inputs, weight, residual, eps, quantized=True)
     return out, scales, (inputs if residual is None else stream_out)

@@ -94,6 +94,13 @@ def _call(dev, entry, *args):
         _lib.check(rc)
 
 
+def _once(gradients, ctx, *grads):
+    """A node's gradients, differentiable once: the guard against a second time is only put up where one could follow.
+    (This runs on autograd's own thread, where every Python object that the forward call has just used is in another
+    core's cache: the arguments are not checked a second time either.)"""
+    return once_differentiable(gradients)(ctx, *grads) if torch.is_grad_enabled() else gradients(ctx, *grads)
+
+
 def _tracked(*tensors):
     """Whether autograd follows a call with these arguments."""
     if not torch.is_grad_enabled():
@@ -133,18 +140,20 @@ def _carried(initial_state, shape, like, dtype):
 
 
 def _conv_forward(inputs, weight, bias, initial_state, lengths, silu, return_state):
-    B, D, L, W, code, flags = _conv_check(inputs, weight, bias, initial_state, lengths, silu)
+    """(out, final state or None, the checked sizes)"""
+    sizes = _conv_check(inputs, weight, bias, initial_state, lengths, silu)
+    B, D, L, W, code, flags = sizes
     out = torch.empty((B, D, L), dtype=inputs.dtype, device=inputs.device)
     if not out.numel():
-        return out, _carried(initial_state, (B, D, W - 1), inputs, inputs.dtype) if return_state else None
+        return out, _carried(initial_state, (B, D, W - 1), inputs, inputs.dtype) if return_state else None, sizes
     final = torch.empty((B, D, W - 1), dtype=inputs.dtype, device=inputs.device) if return_state else None
     _call(inputs.device, _raw.fmselective_conv_forward, inputs.data_ptr(), inputs.stride(0), inputs.stride(1), weight.data_ptr(),
           _ptr(bias), _ptr(initial_state), _ptr(lengths), out.data_ptr(), _ptr(final), B, D, L, W, code, flags)
-    return out, final
+    return out, final, sizes
 
 
-def _conv_backward(inputs, weight, bias, initial_state, lengths, silu, out_grad, final_grad, want_state):
-    B, D, L, W, code, flags = _conv_check(inputs, weight, bias, initial_state, lengths, silu)
+def _conv_backward(inputs, weight, bias, initial_state, lengths, sizes, out_grad, final_grad, want_state):
+    B, D, L, W, code, flags = sizes
     dev = inputs.device
     if out_grad is None:
         out_grad = torch.zeros((B, D, L), dtype=inputs.dtype, device=dev)
@@ -180,20 +189,21 @@ class FM_Conv(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, inputs, weight, bias=None, initial_state=None, lengths=None, silu=True, return_state=False):
+        out, final, ctx.sizes = _conv_forward(inputs, weight, bias, initial_state, lengths, silu, return_state)
         ctx.save_for_backward(inputs, weight, bias, initial_state, lengths)
-        ctx.silu = bool(silu)
         ctx.set_materialize_grads(False)
-        return _conv_forward(inputs, weight, bias, initial_state, lengths, silu, return_state)
+        return out, final
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, out_grad, final_grad):
-        inputs, weight, bias, initial_state, lengths = ctx.saved_tensors
-        if out_grad is None and final_grad is None:
-            return (None,) * 7
-        grads = _conv_backward(inputs, weight, bias, initial_state, lengths, ctx.silu, out_grad, final_grad,
-                               ctx.needs_input_grad[3])
-        return (*grads, None, None, None)
+        return _once(_conv_gradients, ctx, out_grad, final_grad)
+
+
+def _conv_gradients(ctx, out_grad, final_grad):
+    if out_grad is None and final_grad is None:
+        return (None,) * 7
+    grads = _conv_backward(*ctx.saved_tensors, ctx.sizes, out_grad, final_grad, ctx.needs_input_grad[3])
+    return (*grads, None, None, None)
 
 
 def fm_conv(inputs, weight, bias=None, initial_state=None, lengths=None, silu=True, return_state=False):
@@ -215,7 +225,7 @@ def fm_conv(inputs, weight, bias=None, initial_state=None, lengths=None, silu=Tr
     if _tracked(inputs, weight, bias, initial_state):
         out, final = FM_Conv.apply(inputs, weight, bias, initial_state, lengths, silu, return_state)
     else:
-        out, final = _conv_forward(inputs, weight, bias, initial_state, lengths, silu, return_state)
+        out, final, _ = _conv_forward(inputs, weight, bias, initial_state, lengths, silu, return_state)
     return (out, final) if return_state else out
 
 
@@ -280,8 +290,8 @@ def _channels(tokens, delta, A, skip, gate, delta_bias, G, softplus):
     return N, code, flags
 
 
-def _scan_inputs(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus):
-    """The checked arguments of a call on sequences, as the library takes them, and (B, D, L, N, G, dtype code)."""
+def _scan_check(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus):
+    """Checks the arguments of a call on sequences; ((B, D, L, N, G, dtype code), flags)."""
     _gpu("tokens", tokens)
     if tokens.dim() != 3 or A.dim() != 2 or write.dim() != 4:
         _require(False, "tokens must be (B, D, L), A (D, N), write (B, G, N, L)")
@@ -294,12 +304,17 @@ def _scan_inputs(tokens, delta, A, write, read, skip, gate, delta_bias, initial_
         _dense("initial_state", initial_state, (B, D, N), torch.float32, dev)
     if lengths is not None:
         _dense("lengths", lengths, (B,), torch.int32, dev)
+    return (B, D, L, N, G, code), flags
+
+
+def _scan_packed(sizes, flags, tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths):
+    """The arguments as the library takes them."""
+    B, D, L, N, G, code = sizes
     z_b, z_d = (0, 0) if gate is None else gate.stride()[:2]
-    packed = _lib.SCAN_INPUTS.pack(
+    return _lib.SCAN_INPUTS.pack(
         tokens.data_ptr(), delta.data_ptr(), _at(gate), write.data_ptr(), read.data_ptr(), _at(skip), _at(delta_bias),
         A.data_ptr(), _at(initial_state), _at(lengths), *tokens.stride()[:2], *delta.stride()[:2], z_b, z_d,
         *write.stride()[:3], *read.stride()[:3], B, D, L, N, G, code, flags)
-    return packed, (B, D, L, N, G, code)
 
 
 def _at(t):
@@ -307,27 +322,29 @@ def _at(t):
 
 
 def _scan_forward(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus, return_state, save):
-    """(out, final state or None, the states that backward starts from or None)"""
-    packed, sizes = _scan_inputs(tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths, softplus)
+    """(out, final state or None, the states that backward starts from or None, the checked sizes and flags)"""
+    inputs = (tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths)
+    checked = sizes, flags = _scan_check(*inputs, softplus)
     B, D, L, N, G, code = sizes
     dev = tokens.device
     out = torch.empty((B, D, L), dtype=tokens.dtype, device=dev)
     if not (B and D and L):
-        return out, _carried(initial_state, (B, D, N), tokens, torch.float32) if return_state else None, None
+        return out, _carried(initial_state, (B, D, N), tokens, torch.float32) if return_state else None, None, checked
     final = torch.empty((B, D, N), dtype=torch.float32, device=dev) if return_state else None
     marks = None
     if save:
         marks = torch.empty((B, D, -(-L // _lib.SELECTIVE_MARK), N), dtype=torch.float32, device=dev)
     need = _raw.fmselective_scan_workspace_bytes(*sizes, 0)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(dev, _raw.fmselective_scan_forward, packed, out.data_ptr(), _ptr(final), _ptr(marks), _ptr(workspace), need)
-    return out, final, marks
+    _call(dev, _raw.fmselective_scan_forward, _scan_packed(sizes, flags, *inputs), out.data_ptr(), _ptr(final), _ptr(marks),
+          _ptr(workspace), need)
+    return out, final, marks, checked
 
 
-def _scan_backward(inputs, softplus, marks, out_grad, final_grad, want_state):
+def _scan_backward(inputs, checked, marks, out_grad, final_grad, want_state):
     """Gradients in the order of the inputs, None for absent ones."""
     tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths = inputs
-    packed, sizes = _scan_inputs(*inputs, softplus)
+    sizes, flags = checked
     B, D, L, N, G, code = sizes
     dev, dtype = tokens.device, tokens.dtype
     if out_grad is None:
@@ -353,7 +370,7 @@ def _scan_backward(inputs, softplus, marks, out_grad, final_grad, want_state):
     o = _lib.SCAN_GRADS.pack(out_grad.data_ptr(), *out_grad.stride()[:2], _at(final_grad), marks.data_ptr(),
                              d_tokens.data_ptr(), d_delta.data_ptr(), _at(d_gate), d_write.data_ptr(), d_read.data_ptr(),
                              d_A.data_ptr(), _at(d_state), _at(d_skip), _at(d_bias))
-    _call(dev, _raw.fmselective_scan_backward, packed, o, workspace.data_ptr(), need)
+    _call(dev, _raw.fmselective_scan_backward, _scan_packed(sizes, flags, *inputs), o, workspace.data_ptr(), need)
     return (*grads, d_state)
 
 
@@ -367,21 +384,24 @@ class FM_Selective(torch.autograd.Function):
                 softplus=True, return_state=False):
         inputs = (tokens, delta, A, write, read, skip, gate, delta_bias, initial_state, lengths)
         save = any(ctx.needs_input_grad)
-        out, final, marks = _scan_forward(*inputs, softplus, return_state, save)
+        out, final, marks, checked = _scan_forward(*inputs, softplus, return_state, save)
         if save:
             ctx.save_for_backward(*inputs, marks)
-            ctx.softplus = bool(softplus)
+            ctx.checked = checked
         ctx.set_materialize_grads(False)
         return out, final
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, out_grad, final_grad):
-        *inputs, marks = ctx.saved_tensors
-        if out_grad is None and final_grad is None:
-            return (None,) * 12
-        grads = _scan_backward(inputs, ctx.softplus, marks, out_grad, final_grad, ctx.needs_input_grad[8])
-        return (*grads, None, None, None)
+        return _once(_scan_gradients, ctx, out_grad, final_grad)
+
+
+def _scan_gradients(ctx, out_grad, final_grad):
+    if out_grad is None and final_grad is None:
+        return (None,) * 12
+    *inputs, marks = ctx.saved_tensors
+    grads = _scan_backward(inputs, ctx.checked, marks, out_grad, final_grad, ctx.needs_input_grad[8])
+    return (*grads, None, None, None)
 
 
 def fm_selective_scan(tokens, delta, A, write, read, skip=None, gate=None, delta_bias=None, initial_state=None, lengths=None,
@@ -412,7 +432,7 @@ def fm_selective_scan(tokens, delta, A, write, read, skip=None, gate=None, delta
     if _tracked(*inputs):
         out, final = FM_Selective.apply(*inputs, softplus, return_state)
     else:
-        out, final, _ = _scan_forward(*inputs, softplus, return_state, False)
+        out, final, _, _ = _scan_forward(*inputs, softplus, return_state, False)
     return (out, final) if return_state else out
 
 

@@ -759,3 +759,17 @@ def test_calls_from_two_threads(m):
     threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1)]
     [t.start() for t in threads], [t.join() for t in threads]
     assert not bad
+
+
+def test_gradients_are_differentiable_once(m, nm):
+    """create_graph gives the same gradients, and a second derivative is an error, not a wrong number."""
+    g = gen(61)
+    x, w = rand(g, 2, 3, 20).requires_grad_(), rand(g, 3, 4).requires_grad_()
+    n = (1 + rand(g, 20, scale=0.1)).requires_grad_()
+    a, *_ = scan_case((2, 3, 20, 2, 1), F32, 0)
+    for out in (m.fm_conv(x, w), nm.fm_norm(x, n)[0], m.fm_selective_scan(**{**a, "tokens": x})):
+        (once,) = torch.autograd.grad(out.square().sum(), [x], retain_graph=True)
+        (graph,) = torch.autograd.grad(out.square().sum(), [x], create_graph=True)
+        assert torch.equal(once, graph)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            graph.sum().backward()
