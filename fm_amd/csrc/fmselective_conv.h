@@ -132,6 +132,8 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(const T* __restrict__
         for (int j = 0; j < CH; ++j) raw[j] = fmscan::load_chunk<T, false, false>(x, start + (j * 64 + lane) * E, len, 0u);
     }
     float w[W], bv, first[W - 1];
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) first[i] = 0.0f;
     if (lane == 0) values_before<T, W>(x, start, len, state, first);
     conv_taps<T, W>(weight, bias, d, flags, w, bv);
 #pragma unroll

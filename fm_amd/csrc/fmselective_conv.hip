@@ -74,8 +74,8 @@ int fmselective_conv_forward(const void* inputs, int64_t batch_stride, int64_t c
     } else {
         g.units = (g.chunks + 64 * each - 1) / (64 * each);
         blocks = ((int64_t)g.rows * g.units + 3) / 4;
-        if (blocks > INT32_MAX / 4) return fail(FMSCAN_E_SHAPE, "%s: B * D * L is too large for one launch", who);
     }
+    if (int rc = check_grid(who, blocks, 256)) return rc;
     with_dtype(dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
         with_taps(W, [&](auto wt) {
@@ -133,6 +133,8 @@ int fmselective_conv_backward(const void* inputs, int64_t batch_stride, int64_t 
     g.grad_channel_stride = grad_channel_stride;
     const int64_t slots = (int64_t)g.rows * g.segments, per_wave = 64 >> g.lanes_log2;
     const int64_t blocks = ((slots + per_wave - 1) / per_wave + 3) / 4;
+    if (int rc = check_grid(who, blocks, 256)) return rc;
+    if (int rc = check_grid(who, (__int128)D * (W + 1) + 128, 16)) return rc;  // the sums of the parameters' gradients
     float* weight_part = (float*)workspace;
     float* bias_part = weight_part + slots * W;
     with_dtype(dtype, [&](auto tt) {
@@ -174,7 +176,7 @@ int fmselective_conv_step(const void* inputs, int64_t batch_stride, const void* 
     if (state_out != state)
         if (int rc = check_alias(who, {new_r}, {old_r})) return rc;
     const uint32_t tiles = (uint32_t)((D + 1023) / 1024);
-    if ((__int128)B * tiles > (__int128)INT32_MAX) return fail(FMSCAN_E_SHAPE, "%s: B * D is too large for one launch", who);
+    if (int rc = check_grid(who, (__int128)B * tiles, 256)) return rc;
     with_dtype(dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
         with_taps(W, [&](auto wt) {

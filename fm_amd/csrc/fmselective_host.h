@@ -6,6 +6,8 @@
 #include "fmscan_host.h"
 #include "fmselective_device.h"
 
+#include <utility>
+
 namespace fmselective {
 namespace host {
 
@@ -43,9 +45,20 @@ inline int check_pool(const char* who, int64_t S, int64_t B, int64_t each, const
     return 0;
 }
 
-// the bytes between the first and the last element of a strided (B, D, L) tensor
+// the bytes between the first and the last element of a strided tensor (at most 2^62: a range, not a size to allocate)
+inline int64_t span(std::initializer_list<std::pair<int64_t, int64_t>> axes, int esize) {
+    __int128 n = 1;
+    for (const auto& a : axes) n += (__int128)(a.first - 1) * a.second;
+    n *= esize;
+    return n > ((__int128)1 << 62) ? (int64_t)1 << 62 : (int64_t)n;
+}
 inline int64_t extent(int64_t B, int64_t D, int64_t L, int64_t sb, int64_t sd, int esize) {
-    return ((B - 1) * sb + (D - 1) * sd + L) * esize;
+    return span({{B, sb}, {D, sd}, {L, 1}}, esize);
+}
+
+// A launch's threads are counted in 32 bits
+inline int check_grid(const char* who, __int128 blocks, int threads) {
+    return blocks * threads >= ((__int128)1 << 32) ? fail(FMSCAN_E_SHAPE, "%s: these sizes are too large for one launch", who) : 0;
 }
 
 inline int check_alias(const char* who, std::initializer_list<Range> outs, std::initializer_list<Range> ins) {

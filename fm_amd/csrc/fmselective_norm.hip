@@ -61,6 +61,9 @@ int fmselective_norm_forward(const void* inputs, const void* residual, const voi
                              {{"inputs", inputs, rows * D * es}, {"residual", residual, rows * D * es},
                               {"weight", weight, D * (flags & FMSELECTIVE_NARROW_WEIGHT ? es : 4)}}))
         return rc;
+    int threads = 0;  // a row
+    with_row_shape(D, dtype, [&](auto pt, auto) { threads = decltype(pt)::value; });
+    if (int rc = check_grid(who, (__int128)rows + 3, threads)) return rc;
     with_dtype(dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
         with_row_shape(D, dtype, [&](auto pt, auto ct) {

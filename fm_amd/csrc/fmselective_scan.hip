@@ -46,7 +46,7 @@ int launch_forward(const char* who, const fmselective_scan_inputs& in, Cut cut, 
                    void* pairs, hipStream_t stream) {
     const Scan p = scan_of(in, WAVES * 64 / LPC, cut, pairs);
     const int64_t blocks = in.B * in.G * p.blocks_per_group * cut.segments;
-    if (blocks > INT32_MAX) return fail(FMSCAN_E_SHAPE, "%s: B * D is too large for one launch", who);
+    if (int rc = check_grid(who, blocks, 64 * WAVES)) return rc;
     static std::atomic<uint64_t> armed{0}, armed_ends{0};
     const size_t lds = fmselective::scan_forward_lds<LPC, WAVES>(p.N);
     const auto kernel = fmselective::selective_forward_kernel<T, LPC, WAVES, false>;
@@ -118,9 +118,9 @@ int fmselective_scan_step(const fmselective_scan_inputs* in, float* state_out, c
         return fail(FMSCAN_E_NULL, "%s: initial_state (the pool), state_out and out must not be NULL", who);
     const int es = esize_of(in->dtype);
     const int64_t B = in->B, D = in->D, pool = S * D * in->N * 4;
-    auto row = [&](const char* name, const void* p, const int64_t* s) { return Range{name, p, ((B - 1) * s[0] + D) * es}; };
+    auto row = [&](const char* name, const void* p, const int64_t* s) { return Range{name, p, span({{B, s[0]}, {D, 1}}, es)}; };
     auto shared = [&](const char* name, const void* p, const int64_t* s) {
-        return Range{name, p, ((B - 1) * s[0] + (in->G - 1) * s[1] + in->N) * es};
+        return Range{name, p, span({{B, s[0]}, {in->G, s[1]}, {in->N, 1}}, es)};
     };
     const Range out_r = {"out", out, B * D * es}, new_r = {"state_out", state_out, pool}, old_r = {"the pool", in->initial_state, pool};
     if (int rc = check_alias(who, {out_r, new_r},
@@ -146,7 +146,7 @@ int fmselective_scan_step(const fmselective_scan_inputs* in, float* state_out, c
     const bool many = B * ((D + 63) / 64) >= kManyStepBlocks;
     p.tiles = (uint32_t)(many ? (D + 127) / 128 : (D + 63) / 64);
     p.flags = in->flags;
-    if ((__int128)B * p.tiles > (__int128)INT32_MAX) return fail(FMSCAN_E_SHAPE, "%s: B * D is too large for one launch", who);
+    if (int rc = check_grid(who, (__int128)B * p.tiles, 256)) return rc;
     const bool vec = in->N % 4 == 0 && aligned16(in->A) && aligned16(in->initial_state) && aligned16(state_out);
     with_dtype(in->dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;

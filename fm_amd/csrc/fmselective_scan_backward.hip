@@ -89,8 +89,11 @@ int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselecti
     float* const pairs = (float*)workspace + b.shared;
     const Scan p = scan_of(*in, 4 * kBackWaves, b.cut, pairs);
     const int64_t lines = in->B * in->G * in->N, items = lines * p.marks, blocks = b.blocks * b.cut.segments;
-    if (blocks > INT32_MAX || items > INT32_MAX - (1 << 24))
-        return fail(FMSCAN_E_SHAPE, "%s: B * D or B * G * N * L is too large for one launch", who);
+    if (int rc = check_grid(who, blocks, 64 * kBackWaves)) return rc;
+    int per = 1;  // waves that share a sum of the last launch: at least four terms each
+    while (per < fmselective::kSumWaves && p.blocks_per_group >= 8 * per) per *= 2;
+    // (its threads: 64 a wave and a sum, and 16 a column of the parameters' gradients, three sections of whole blocks)
+    if (int rc = check_grid(who, ((__int128)items * per + 64) * 64 + ((__int128)in->D * in->N + 2 * in->D + 256) * 16, 1)) return rc;
     float* part = (float*)workspace;
     ScanGrads g = {};
     g.out_grad = o.out_grad;
@@ -118,8 +121,6 @@ int fmselective_scan_backward(const fmselective_scan_inputs* in, const fmselecti
              {g.skip_part, o.skip, in->B * b.cut.segments, in->D, (in->flags & FMSELECTIVE_NARROW_SKIP) != 0, 0},
              {g.bias_part, o.delta_bias, in->B * b.cut.segments, in->D, (in->flags & FMSELECTIVE_NARROW_BIAS) != 0, 0}}, &columns);
         constexpr int W = fmselective::kSumWaves;
-        int per = 1;  // waves that share a sum: at least four terms each
-        while (per < W && p.blocks_per_group >= 8 * per) per *= 2;
         fmselective::selective_sums_kernel<T><<<(unsigned)(column_blocks + (items * per + W - 1) / W), 64 * W, 0, st>>>(
             columns, column_blocks, part, (T*)o.write, (T*)o.read, in->lengths, in->L, items, p.N, p.G, p.marks,
             p.blocks_per_group, per);

@@ -84,7 +84,7 @@ inline InputRanges input_ranges(const fmselective_scan_inputs& in) {
     const int es = esize_of(in.dtype);
     auto seq = [&](const char* name, const void* p, const int64_t* s) { return Range{name, p, extent(in.B, in.D, in.L, s[0], s[1], es)}; };
     auto shared = [&](const char* name, const void* p, const int64_t* s) {
-        return Range{name, p, ((in.B - 1) * s[0] + (in.G - 1) * s[1] + (in.N - 1) * s[2] + in.L) * es};
+        return Range{name, p, span({{in.B, s[0]}, {in.G, s[1]}, {in.N, s[2]}, {in.L, 1}}, es)};
     };
     return {{seq("tokens", in.tokens, in.tokens_strides), seq("delta", in.delta, in.delta_strides),
              seq("gate", in.gate, in.gate_strides), shared("write", in.write, in.write_strides),

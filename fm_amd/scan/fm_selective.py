@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 from .fm_scan import _DTYPES, _dtype_code, _on_gpu, _ptr, _raw, _require
@@ -76,10 +77,13 @@ def _pool(state, state_out, slots, B, D, each, dtype, dev):
     _dense("state", state, (S, D, each), dtype, dev)
     if slots is None and S != B:
         _require(False, f"without slots the state must hold {B} rows, got {S}")
-    if state_out is None:
-        return state
-    _dense("state_out", state_out, (S, D, each), dtype, dev)
-    return state_out
+    new = state
+    if state_out is not None:
+        _dense("state_out", state_out, (S, D, each), dtype, dev)
+        new = state_out
+    if not new.is_inference():
+        increment_version(new)  # a graph that holds the states as they were refuses its backward pass
+    return new
 
 
 def _call(dev, entry, *args):
@@ -414,7 +418,8 @@ def fm_selective_scan(tokens, delta, A, write, read, skip=None, gate=None, delta
 
     Arguments:
         tokens, delta (B, D, L) and gate (B, D, L) or None: one dtype, time stride 1, any batch and channel stride.
-        A (D, N): float32, negative in a model whose states decay; N up to 256.
+        A (D, N): float32, negative in a model whose states decay; N up to 256. Where a state grows, its growth over the
+            call's steps must be finite in float32, even while the state itself is zero.
         write, read (B, G, N, L), or (B, N, L) for one group: of the tokens' dtype, time stride 1; channel d is in
             group g = d // (D / G).
         skip, delta_bias (D,): float32 or the tokens' dtype; absent is zero.

@@ -74,7 +74,8 @@ int fmselective_conv_step(const void* inputs, int64_t batch_stride, const void* 
  *   out[b,d,t] = (sum_n read[b,g,n,t] h[b,d,n] + skip[d] tokens[b,d,t]) * silu(gate[b,d,t])
  * with channel d in group g = d / (D / G). tokens, delta, gate (B, D, L) and write, read (B, G, N, L) have one
  * element type and any strides but the time's, which is 1; A (D, N), states and their gradients are float32.
- * gate, skip, delta_bias, initial_state and lengths may be NULL. 1 <= N <= FMSELECTIVE_MAX_STATES, G divides D. */
+ * gate, skip, delta_bias, initial_state and lengths may be NULL. 1 <= N <= FMSELECTIVE_MAX_STATES, G divides D.
+ * Products of decays over many steps are taken: where A is positive they must stay finite in float32. */
 #define FMSELECTIVE_MAX_STATES 256
 #define FMSELECTIVE_MARK 128 /* steps between the states that forward saves for backward */
 

@@ -387,6 +387,29 @@ def test_selective_step_views(m):
     assert torch.equal(state, kept)
 
 
+def test_steps_are_seen_by_a_graph_that_holds_the_states(m):
+    """States that an eager graph keeps for its backward pass and that a step then moves on."""
+    g = gen(22)
+    a = scan_case((2, 4, 9, 3, 1), F32, 0)[0]
+    state = rand(g, 2, 4, 3)
+    tokens = a["tokens"].requires_grad_()
+    y = m.fm_selective_scan(tokens, a["delta"], a["A"], a["write"], a["read"], initial_state=state)
+    token, delta, write, read = (t[..., 0].detach().contiguous() for t in (tokens, a["delta"], a["write"], a["read"]))
+    m.fm_selective_step(token, state, delta, a["A"], write, read)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    carried, w = rand(g, 2, 4, 3), rand(g, 4, 4)
+    y = m.fm_conv(tokens, w, initial_state=carried)
+    other = torch.empty_like(carried)
+    m.fm_conv_step(rand(g, 2, 4), carried, w, state_out=other)  # leaves `carried` as it is
+    y.sum().backward(retain_graph=True)
+    m.fm_conv_step(rand(g, 2, 4), carried, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        m.fm_conv_step(rand(g, 2, 4), rand(g, 2, 4, 3), w)
+
+
 # ---- norm -------------------------------------------------------------------------------------------
 # sum of squares: at most 4 chunks of 8 in a thread and 10 levels, halved by the root; a few operations after it: c = 40
 # the row's second sum, of products: c = 80; weight's gradient: a rounding a row in a slot (8 to rows / 512), then
@@ -449,6 +472,14 @@ def test_norm_quantized_rows_without_a_scale(nm):
     assert torch.isnan(s[3]) and torch.isnan(q[3].float()).all() and torch.isnan(s[4]) and torch.isnan(q[4, 9].float())
     for i in (0, 5):
         assert torch.equal(q[i].float(), alone[0][i].float()) and s[i] == alone[1][i]
+
+
+def test_norm_of_a_subnormal_mean(nm):
+    """Without eps, values whose mean square is subnormal: squares near 2^-132 are off by 2^-150, the root by half of that."""
+    x = torch.randn(3, 300, generator=gen(5)) * 2.0 ** -66
+    y, _ = nm.fm_norm(x.to(DEV), torch.ones(300, device=DEV), eps=0.0)
+    exact = x.double() / x.double().pow(2).mean(-1, keepdim=True).sqrt()
+    assert ((y.cpu().double() - exact).abs() <= 2.0 ** -17 * exact.abs()).all()
 
 
 def test_norm_uses_of_its_outputs(nm):

@@ -180,6 +180,10 @@ def test_scan_rejects(lib):
 
     assert step(state=None) == code("NULL") and step(out=None) == code("NULL")
     assert step(S=3) == code("SHAPE") and step(S=0, slots=16 * P) == code("SHAPE") and step(new=6 * P + 16) == code("ALIAS")
+    # more threads than a launch counts, and strides whose span passes 64 bits
+    assert step(B=1 << 24, S=1 << 24, new=1 << 50, out=1 << 52, state=1 << 50) == code("SHAPE")
+    assert b"one launch" in lib.fmscan_last_error()
+    assert fwd(B=1 << 20, tokens_strides=(1 << 44, 8), out=P + (1 << 50)) == code("ALIAS")
     assert step(out=6 * P) == code("ALIAS") and step(N=300) == code("SHAPE") and step(flags=0x8) == code("FLAGS")
 
 
@@ -191,6 +195,7 @@ def test_norm_rejects(lib):
     assert fwd(eps=-1.0) == code("SHAPE") and fwd(eps=float("nan")) == code("SHAPE") and fwd(dtype=9) == code("DTYPE")
     assert fwd(flags=1) == code("FLAGS") and fwd(out=P) == code("ALIAS") and fwd(r=4 * P, ro=4 * P) == code("ALIAS")
     assert fwd(s=3 * P + 8) == code("ALIAS") and fwd(inv=2 * P) == code("ALIAS")
+    assert fwd(rows=1 << 25, D=4096, x=P, out=1 << 50, w=1 << 52) == code("SHAPE") and b"one launch" in lib.fmscan_last_error()
 
     def bwd(dy=P, dr=None, x=2 * P, w=3 * P, inv=4 * P, g=5 * P, dw=6 * P, ws=7 * P, n=1 << 20):
         return lib.fmselective_norm_backward(dy, dr, x, w, inv, g, dw, 4, 8, 2, 0, ws, n, None)
