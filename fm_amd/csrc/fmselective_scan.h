@@ -51,6 +51,7 @@ struct Scan {
 #define FMSELECTIVE_LEVEL(A, B, CTRL)                     \
     "v_fmac_f32_dpp " B ", " B ", " A " " CTRL "\n\t"     \
     "v_mul_f32_dpp " A ", " A ", " A " " CTRL "\n\t"
+#define FMSELECTIVE_LAST(A, B, CTRL) "v_fmac_f32_dpp " B ", " B ", " A " " CTRL "\n\t"
 template <int LPC>
 __device__ __forceinline__ void scan_up(float& a, float& b) {
     if constexpr (LPC == 16)
@@ -58,7 +59,7 @@ __device__ __forceinline__ void scan_up(float& a, float& b) {
             FMSELECTIVE_LEVEL("%0", "%1", "row_shr:1 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
             FMSELECTIVE_LEVEL("%0", "%1", "row_shr:2 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
             FMSELECTIVE_LEVEL("%0", "%1", "row_shr:4 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
-            FMSELECTIVE_LEVEL("%0", "%1", "row_shr:8 row_mask:0xf bank_mask:0xf")
+            FMSELECTIVE_LAST("%0", "%1", "row_shr:8 row_mask:0xf bank_mask:0xf")
             "s_nop 1"
             : "+v"(a), "+v"(b));
     else
@@ -68,7 +69,7 @@ __device__ __forceinline__ void scan_up(float& a, float& b) {
             FMSELECTIVE_LEVEL("%0", "%1", "row_shr:4 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
             FMSELECTIVE_LEVEL("%0", "%1", "row_shr:8 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
             FMSELECTIVE_LEVEL("%0", "%1", "row_bcast:15 row_mask:0xa bank_mask:0xf") "s_nop 0\n\t"
-            FMSELECTIVE_LEVEL("%0", "%1", "row_bcast:31 row_mask:0xc bank_mask:0xf")
+            FMSELECTIVE_LAST("%0", "%1", "row_bcast:31 row_mask:0xc bank_mask:0xf")
             "s_nop 1"
             : "+v"(a), "+v"(b));
 }
@@ -77,7 +78,7 @@ __device__ __forceinline__ void scan_down(float& a, float& b) {
         FMSELECTIVE_LEVEL("%0", "%1", "row_shl:1 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
         FMSELECTIVE_LEVEL("%0", "%1", "row_shl:2 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
         FMSELECTIVE_LEVEL("%0", "%1", "row_shl:4 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
-        FMSELECTIVE_LEVEL("%0", "%1", "row_shl:8 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LAST("%0", "%1", "row_shl:8 row_mask:0xf bank_mask:0xf")
         "s_nop 1"
         : "+v"(a), "+v"(b));
 }
@@ -91,12 +92,13 @@ __device__ __forceinline__ void scan_both(float& up_a, float& up_b, float& down_
         FMSELECTIVE_LEVEL("%2", "%3", "row_shl:2 row_mask:0xf bank_mask:0xf")
         FMSELECTIVE_LEVEL("%0", "%1", "row_shr:4 row_mask:0xf bank_mask:0xf")
         FMSELECTIVE_LEVEL("%2", "%3", "row_shl:4 row_mask:0xf bank_mask:0xf")
-        FMSELECTIVE_LEVEL("%0", "%1", "row_shr:8 row_mask:0xf bank_mask:0xf")
-        FMSELECTIVE_LEVEL("%2", "%3", "row_shl:8 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LAST("%0", "%1", "row_shr:8 row_mask:0xf bank_mask:0xf")
+        FMSELECTIVE_LAST("%2", "%3", "row_shl:8 row_mask:0xf bank_mask:0xf")
         "s_nop 1"
         : "+v"(up_a), "+v"(up_b), "+v"(down_a), "+v"(down_b));
 }
 #undef FMSELECTIVE_LEVEL
+#undef FMSELECTIVE_LAST
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -346,11 +348,11 @@ __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T
                 float S = v[0], P = exp2_fast(total_dt * e.x);
 #pragma unroll
                 for (int k = 1; k < kSteps; ++k) S = __builtin_fmaf(a[k], S, v[k]);
+                S = __builtin_fmaf(P, c == 0 ? e.y : 0.0f, S);  // the first lane starts from the state that enters the tile
                 scan_up<LPC>(P, S);
-                constexpr int kShift = LPC == 16 ? kRowShr1 : fmscan::kWaveShr1;
-                float h = __builtin_fmaf(fmscan::dpp<kShift>(1.0f, P), e.y, fmscan::dpp<kShift>(0.0f, S));
-                if (c == LPC - 1) state->y = __builtin_fmaf(P, e.y, S);
+                if (c == LPC - 1) state->y = S;
                 if (ENDS) continue;
+                float h = fmscan::dpp<LPC == 16 ? kRowShr1 : fmscan::kWaveShr1>(e.y, S);
                 if (LPC == 64 && marks && (c & 15) == 0) {
                     const int32_t mark = tile * (LPC / 16) + c / 16;
                     if (valid && mark < p.marks) marks[(row * p.marks + mark) * p.N + n0 + n] = h;
@@ -541,19 +543,20 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
                 float S = 0.0f, P = exp2_fast(total_dt * e.x), D = dh[kSteps - 1], Q = P;
 #pragma unroll
                 for (int k = kSteps - 1; k > 0; --k) D = __builtin_fmaf(a[k], D, dh[k - 1]);
-                D *= a[0];
+                D = __builtin_fmaf(Q, c == LPC - 1 ? e.y : 0.0f, a[0] * D);  // the last lane starts from what arrives
                 if constexpr (ENDS) {
                     scan_down(Q, D);
-                    if (c == 0) state->y = __builtin_fmaf(Q, e.y, D);
+                    if (c == 0) state->y = D;
                     continue;
                 }
                 S = h[0];
 #pragma unroll
                 for (int k = 1; k < kSteps; ++k) S = __builtin_fmaf(a[k], S, h[k]);
+                S = __builtin_fmaf(P, c == 0 ? e.w : 0.0f, S);
                 scan_both(P, S, Q, D);
-                const float enter = __builtin_fmaf(fmscan::dpp<kRowShr1>(1.0f, P), e.w, fmscan::dpp<kRowShr1>(0.0f, S));
-                float back = __builtin_fmaf(fmscan::dpp<fmscan::kRowShl1>(1.0f, Q), e.y, fmscan::dpp<fmscan::kRowShl1>(0.0f, D));
-                if (c == 0) state->y = __builtin_fmaf(Q, e.y, D);
+                const float enter = fmscan::dpp<kRowShr1>(e.w, S);
+                float back = fmscan::dpp<fmscan::kRowShl1>(e.y, D);
+                if (c == 0) state->y = D;
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
                     h[k] = __builtin_fmaf(a[k], k ? h[k - 1] : enter, h[k]);
