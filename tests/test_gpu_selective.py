@@ -50,7 +50,8 @@ def spoil(t, lengths):
 # in a lane (L / 64 + 8), the lanes' tree and the column sums (6 + B segments / 8 + 8)
 
 CONV_SHAPES = [(1, 1, 1, 2), (2, 3, 2, 4), (1, 5, 3, 3), (3, 7, 8, 4), (2, 4, 9, 2), (2, 3, 64, 4), (2, 65, 127, 3),
-               (1, 3, 511, 4), (2, 2, 513, 4), (1, 2, 2049, 4), (1, 1, 9000, 4), (700, 3, 5, 4)]
+               (1, 3, 511, 4), (2, 2, 513, 4), (1, 2, 2049, 4), (1, 1, 9000, 4), (700, 3, 5, 4),
+               (170, 6400, 1, 3), (500, 640, 9, 4), (330, 210, 65, 2)]
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])

@@ -50,6 +50,7 @@ def test_conv_rejects(lib):
     assert fwd(dtype=3) == code("DTYPE") and fwd(flags=1) == code("FLAGS") and fwd(flags=0x100) == code("FLAGS")
     assert fwd(out=P + 16) == code("ALIAS") and fwd(f=3 * P + 8) == code("ALIAS") and fwd(s=4 * P, f=4 * P) == code("ALIAS")
     assert b"overlaps" in lib.fmscan_last_error()
+    assert fwd(out=2 * P + 2 * 3 * 4) == code("ALIAS") and fwd(bias=3 * P - 8) == code("ALIAS")  # float32 parameters: 48 and 12 bytes
     need = lib.fmselective_conv_workspace_bytes
     assert need(2, 3, 8, 4, 2) == 2 * 3 * 5 * 4 and need(2, 3, 8, 5, 2) == 0 and need(2, 3, 0, 4, 2) == 0
 
