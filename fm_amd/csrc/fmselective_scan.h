@@ -10,8 +10,15 @@
 // of 128 steps, so a wave works on 4 channels at a time and every tensor moves as 16-byte accesses along time.
 // For one state of a channel a lane composes its 8 steps (its total decay is one exponential of the steps' sum),
 // the row scans the pairs (decay, value) by DPP, and a second walk over the 8 steps with the true entering state
-// gives the states. A block's waves share the tile of write and read, kept in LDS as float32 and fetched one
-// tile ahead; the state that leaves a tile waits in LDS for the next one.
+// gives the states; the state that enters the tile joins the scan in its first lane. A block's waves share the tile of
+// write and read, kept in LDS as float32 and loaded while the tile before is worked on; the state that leaves a tile
+// waits in LDS for the next one.
+//
+// Tried and not taken, at (8, 2048, 2048) with N = 16 in bf16: the exponents dt A as outer products of the matrix units
+// (registers: forward 205 -> 220 to 300 us, backward 605 -> 830); two sets of channels a lane in backward (328 registers,
+// 606 -> 748 us); more waves a SIMD by a bound on registers (spills, 591 -> 660 to 750); two states a turn in forward
+// (142 registers, 196 -> 214 us; bounded to 128 it spills, 208); blocks of 8 waves in backward (618 + 27 against
+// 591 + 49 us).
 #pragma once
 
 #include "fmselective_device.h"
@@ -241,6 +248,9 @@ __device__ __forceinline__ void steps_of(float (&dt)[kSteps], float bias, uint32
 // Forward over the tiles of a segment. Where rows are too few to fill the GPU they are cut into segments: a first
 // launch (ENDS) finds what each segment but the last does to a state, without the outputs; the second composes
 // the segments before its own, as many multiply-adds a state, and then runs as for a whole row.
+// Bound by vector instructions: a state and step is 8 of them (two walks of 8 steps, the scan between them, the exponential
+// at half rate) and 3 more are the steps' own softplus, gate and conversions. With N = 16 in bf16 196 us at (8, 2048, 2048),
+// 2.7e12 states a second, the SIMDs busy for 90 % of it; 409 us at (1, 4096, 16384), 2.6e12.
 template <typename T, int LPC, int WAVES, bool ENDS>
 __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T* __restrict__ out, float* __restrict__ final_state,
                                                                        float* __restrict__ marks) {
@@ -433,6 +443,8 @@ size_t scan_backward_lds(int N) {
 // blocks by a second kernel, always in the same order.
 // Rows that are too few to fill the GPU are cut into segments, as in forward: the first launch (ENDS) finds what each
 // segment but the first hands on of a gradient that enters it from behind.
+// Bound by vector instructions, about 29 a state and step, at two waves a SIMD (237 registers): 553 us at (8, 2048, 2048),
+// N = 16 in bf16, the SIMDs busy for 85 % of it. What it leaves for the sums over the channels is 268 MB there.
 template <typename T, int WAVES, bool ENDS>
 __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, ScanGrads o) {
     constexpr int LPC = 16, NC = 16, kTile = LPC * kSteps;
@@ -683,7 +695,7 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
 // The last sums of a backward call, in one launch. The first blocks take the parameters' gradients (column_sums); the
 // others the gradients of write and read: the partial sums added up in a fixed order and rounded once, `per` waves of
 // a block for one (b, g, n, mark), each every per-th partial sum, a float4 a lane, in the order that the backward
-// kernel left them.
+// kernel left them. Bound by memory: 62 us for 268 MB at (8, 2048, 2048), N = 16, 4.4 TB/s.
 template <typename T>
 __global__ __launch_bounds__(64 * kSumWaves) void selective_sums_kernel(ColumnSums columns, uint32_t column_blocks,
                                                                         const float* __restrict__ part, T* __restrict__ write_grad,
@@ -740,7 +752,8 @@ struct Step {
 // One token: four lanes a channel, each takes every fourth group of four states, 16 bytes at a time where N allows;
 // a block takes 64 channels of a row, CH times. The row's `write` and `read` serve all its channels of a group.
 // Bound by the pool's traffic: what does not depend on the slot is loaded before it is known, and the new states, which
-// this call does not read again, are stored past the caches (47 -> 35 us at 256 rows of 4096 channels with 16 states).
+// this call does not read again, are stored past the caches (47 -> 35 us at 256 rows of 4096 channels with 16 states;
+// 29 us, 4.9 TB/s, with two channels a lane). 3.1 us at one row of 2048.
 template <typename T, bool VEC, int CH>
 __global__ __launch_bounds__(256) void selective_step_kernel(Step p, T* __restrict__ out) {
     const uint32_t b = p.tiles == 1 ? blockIdx.x : blockIdx.x / p.tiles;
