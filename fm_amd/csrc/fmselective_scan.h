@@ -7,7 +7,8 @@
 // (b, d, t). With 16 states the kernels are bound by vector float32 arithmetic, not by memory.
 //
 // Layout. Time runs along the lanes: a lane holds 8 consecutive steps of a channel, 16 lanes (one DPP row) a tile
-// of 128 steps, so a wave works on 4 channels at a time and every tensor moves as 16-byte accesses along time.
+// of 128 steps, so a wave works on 4 channels at a time and every tensor moves as 16-byte accesses along time. (Forward
+// also has tiles of 4 lanes, 32 steps of 16 channels, and of 64, 512 steps of one.)
 // For one state of a channel a lane composes its 8 steps (its total decay is one exponential of the steps' sum),
 // the row scans the pairs (decay, value) by DPP, and a second walk over the 8 steps with the true entering state
 // gives the states; the state that enters the tile joins the scan in its first lane. A block's waves share the tile of
@@ -61,7 +62,14 @@ struct Scan {
 #define FMSELECTIVE_LAST(A, B, CTRL) "v_fmac_f32_dpp " B ", " B ", " A " " CTRL "\n\t"
 template <int LPC>
 __device__ __forceinline__ void scan_up(float& a, float& b) {
-    if constexpr (LPC == 16)
+    if constexpr (LPC == 4) {  // by quad permutations, which bring a lane no other channel's values
+        const int c = threadIdx.x & 3;
+        const float pb = fmscan::dpp<0x90>(0.0f, b), pa = fmscan::dpp<0x90>(0.0f, a);  // lanes 0, 0, 1, 2
+        b = c ? __builtin_fmaf(pb, a, b) : b;
+        a = c ? pa * a : a;
+        const float qb = fmscan::dpp<0x44>(0.0f, b);  // lanes 0, 1, 0, 1
+        b = c & 2 ? __builtin_fmaf(qb, a, b) : b;
+    } else if constexpr (LPC == 16)
         asm("s_nop 1\n\t"
             FMSELECTIVE_LEVEL("%0", "%1", "row_shr:1 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
             FMSELECTIVE_LEVEL("%0", "%1", "row_shr:2 row_mask:0xf bank_mask:0xf") "s_nop 0\n\t"
@@ -108,6 +116,15 @@ __device__ __forceinline__ void scan_both(float& up_a, float& up_b, float& down_
 #undef FMSELECTIVE_LAST
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// The value of the lane below of the same channel, in its first lane `first`
+template <int LPC>
+__device__ __forceinline__ float of_lane_below(float first, float v) {
+    if constexpr (LPC == 4) {
+        const float below = fmscan::dpp<0x90>(0.0f, v);  // (by all lanes: none reads an inactive one)
+        return threadIdx.x & 3 ? below : first;
+    } else return fmscan::dpp<LPC == 16 ? 0x111 : fmscan::kWaveShr1>(first, v);  // row_shr 1
+}
 
 constexpr int kRowShr1 = 0x111;  // lane i <- lane i-1 inside its row of 16
 
@@ -201,7 +218,7 @@ __host__ __device__ __forceinline__ int state_stride(int N) { return N | 1; }
 
 // Forward keeps two tiles of kStates states in LDS (one being filled), backward one
 template <int LPC, int WAVES>
-constexpr int tile_states() { return LPC == 16 ? 16 : WAVES; }
+constexpr int tile_states() { return LPC == 64 ? WAVES : LPC == 16 ? 16 : 32; }
 template <int LPC, int WAVES>
 size_t scan_forward_lds(int N) {
     return 2 * sizeof(SharedTile<LPC, tile_states<LPC, WAVES>()>) + (size_t)WAVES * (64 / LPC) * state_stride(N) * sizeof(float2);
@@ -254,6 +271,7 @@ __device__ __forceinline__ void steps_of(float (&dt)[kSteps], float bias, uint32
 template <typename T, int LPC, int WAVES, bool ENDS>
 __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T* __restrict__ out, float* __restrict__ final_state,
                                                                        float* __restrict__ marks) {
+    static_assert(LPC == 64 || !ENDS, "only rows of 64 lanes are cut");
     constexpr int NC = tile_states<LPC, WAVES>(), kTile = LPC * kSteps, CW = 64 / LPC;
     using Tile = SharedTile<LPC, NC>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -336,8 +354,9 @@ __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T
             if (tile + 1 < n_tiles) fetch_rows(tile + 1);
         }
         if (ENDS) all_dt += total_dt;
-        if (LPC == 16 && !ENDS && marks && valid) {
-            float* mark = marks + (row * p.marks + tile) * p.N;
+        constexpr int kMarkTiles = kTile < kMark ? kMark / kTile : 1;
+        if (LPC != 64 && !ENDS && marks && valid && tile % kMarkTiles == 0) {
+            float* mark = marks + (row * p.marks + tile / kMarkTiles) * p.N;
             for (int n = c; n < p.N; n += LPC) mark[n] = held[n].y;
         }
         for (int chunk = 0; chunk < chunks; ++chunk, ++it) {
@@ -362,7 +381,7 @@ __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T
                 scan_up<LPC>(P, S);
                 if (c == LPC - 1) state->y = S;
                 if (ENDS) continue;
-                float h = fmscan::dpp<LPC == 16 ? kRowShr1 : fmscan::kWaveShr1>(e.y, S);
+                float h = of_lane_below<LPC>(e.y, S);
                 if (LPC == 64 && marks && (c & 15) == 0) {
                     const int32_t mark = tile * (LPC / 16) + c / 16;
                     if (valid && mark < p.marks) marks[(row * p.marks + mark) * p.N + n0 + n] = h;
@@ -393,11 +412,8 @@ __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T
     if constexpr (ENDS) {
         // (the total's decay in one exponential of the summed steps, as within a tile)
         all_dt = row_sum(all_dt);
-        if constexpr (LPC == 64)
-            all_dt = fmscan::lane_value(all_dt, 15) + fmscan::lane_value(all_dt, 31) + fmscan::lane_value(all_dt, 47) +
-                     fmscan::lane_value(all_dt, 63);
-        else
-            all_dt = __shfl(all_dt, lane | 15);
+        all_dt = fmscan::lane_value(all_dt, 15) + fmscan::lane_value(all_dt, 31) + fmscan::lane_value(all_dt, 47) +
+                 fmscan::lane_value(all_dt, 63);
         if (valid)
             for (int n = c; n < p.N; n += LPC)
                 p.pairs[((int64_t)w.seg * p.rows + row) * p.N + n] = make_float2(exp2_fast(all_dt * held[n].x), held[n].y);

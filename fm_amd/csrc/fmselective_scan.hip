@@ -6,11 +6,13 @@ using fmselective::Scan;
 
 namespace {
 
-// Lanes a channel: 16, so that a wave works on 4 channels, or all 64, so that four times as many waves work on tiles of
-// four times the length. Measured for N = 16, bf16, on tiles of one wave: with up to two waves a SIMD a tile takes 5 to
-// 7 us of 16 lanes (128 steps of four channels) and 7 to 8 us of 64 (512 of one), the instructions' latency; with more
-// it is their number that counts, 3.1 and 3.5 us for each of a SIMD's waves. The faster of the two by that is taken:
-// (7, 1024, 515) 57 -> 40 us with 16 lanes, (1, 4096, 16384) 680 -> 440 with 64, (1, 4096, 500) 26 -> 20.
+// Lanes a channel: 16, so that a wave works on 4 channels, all 64, so that four times as many waves work on tiles of
+// four times the length, or 4, so that a quarter as many work on tiles of 32 steps. Measured for N = 16, bf16, on tiles of
+// one wave: with up to two waves a SIMD a tile takes 5 to 7 us of 16 lanes (128 steps of four channels) or of 4 (32 of 16)
+// and 7 to 8 us of 64 (512 of one), the instructions' latency; with more it is their number that counts, 3.1, 3.9 and
+// 3.5 us for each of a SIMD's waves. The fastest by that is taken: (7, 1024, 515) 57 -> 40 us with 16 lanes against 64,
+// (1, 4096, 16384) 680 -> 440 with 64 against 16, (1, 4096, 500) 26 -> 20; with 4 against 16 lanes (64, 4096, 8) 170 -> 51,
+// (32, 2048, 64) 47 -> 28, (16, 4096, 150) 91 -> 69, but (8, 4096, 200) 47 -> 52, (16, 4096, 100) 55 both.
 // Where 64 lanes leave less than two waves a SIMD the rows are cut, for four: (1, 1024, 16384) 225 -> 179 us,
 // (1, 512, 16384) 112 -> 95 (against a cut for two).
 constexpr int64_t kSimds = 1024;
@@ -32,11 +34,14 @@ struct ForwardPlan {
 };
 ForwardPlan plan_forward(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G) {
     ForwardPlan f;
-    const int64_t waves16 = B * G * ((D / G + 3) / 4), waves64 = B * D;
-    const int64_t tiles16 = (L + 127) / 128, tiles64 = (L + 511) / 512;
-    f.lanes = modelled_time(tiles16, waves16, 65, 31) <= modelled_time(tiles64, waves64, 75, 35) ? 16 : 64;
-    // (16 lanes are only taken where the rows are short or many: not cut)
-    f.cut = f.lanes == 16 ? Cut{1, (int32_t)tiles16} : cut_of(tiles64, waves64, waves64 < kCutBelow ? kCutWant : waves64);
+    const int64_t waves4 = B * G * ((D / G + 15) / 16), waves16 = B * G * ((D / G + 3) / 4), waves64 = B * D;
+    const int64_t tiles4 = (L + 31) / 32, tiles16 = (L + 127) / 128, tiles64 = (L + 511) / 512;
+    const int64_t time4 = modelled_time(tiles4, waves4, 65, 39), time16 = modelled_time(tiles16, waves16, 65, 31);
+    f.lanes = time16 <= modelled_time(tiles64, waves64, 75, 35) ? 16 : 64;
+    if (f.lanes == 16 && time4 < time16) f.lanes = 4;
+    // (4 or 16 lanes are only taken where the rows are short or many: not cut)
+    f.cut = f.lanes == 4 ? Cut{1, (int32_t)tiles4} : f.lanes == 16 ? Cut{1, (int32_t)tiles16}
+                         : cut_of(tiles64, waves64, waves64 < kCutBelow ? kCutWant : waves64);
     f.bytes = f.cut.segments > 1 ? (size_t)(f.cut.segments - 1) * B * D * N * sizeof(float2) : 0;
     return f;
 }
@@ -50,16 +55,18 @@ int launch_forward(const char* who, const fmselective_scan_inputs& in, Cut cut, 
     static std::atomic<uint64_t> armed{0}, armed_ends{0};
     const size_t lds = fmselective::scan_forward_lds<LPC, WAVES>(p.N);
     const auto kernel = fmselective::selective_forward_kernel<T, LPC, WAVES, false>;
-    const auto ends = fmselective::selective_forward_kernel<T, LPC, WAVES, true>;
-    if (lds > 64 * 1024) {
+    if (lds > 64 * 1024)
         if (int rc = raise_lds_limit((const void*)kernel, armed, who)) return rc;
-        if (int rc = raise_lds_limit((const void*)ends, armed_ends, who)) return rc;
-    }
-    if (cut.segments > 1) {
-        Scan q = p;  // every segment but the last
-        q.segments = cut.segments - 1;
-        ends<<<(unsigned)(blocks / cut.segments * q.segments), 64 * WAVES, lds, stream>>>(q, (T*)nullptr, nullptr, nullptr);
-        if (int rc = launched("selective scan (ends of segments)")) return rc;
+    if constexpr (LPC == 64) {
+        if (cut.segments > 1) {
+            const auto ends = fmselective::selective_forward_kernel<T, LPC, WAVES, true>;
+            if (lds > 64 * 1024)
+                if (int rc = raise_lds_limit((const void*)ends, armed_ends, who)) return rc;
+            Scan q = p;  // every segment but the last
+            q.segments = cut.segments - 1;
+            ends<<<(unsigned)(blocks / cut.segments * q.segments), 64 * WAVES, lds, stream>>>(q, (T*)nullptr, nullptr, nullptr);
+            if (int rc = launched("selective scan (ends of segments)")) return rc;
+        }
     }
     kernel<<<(unsigned)blocks, 64 * WAVES, lds, stream>>>(p, (T*)out, final_state, marks);
     return launched("selective scan (forward)");
@@ -100,8 +107,8 @@ int fmselective_scan_forward(const fmselective_scan_inputs* in, void* out, float
     with_dtype(in->dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
         constexpr int W = fmselective::kScanWaves;
-        rc = f.lanes == 16 ? launch_forward<T, 16, W>(who, *in, f.cut, out, final_state, marks, workspace, (hipStream_t)stream)
-                           : launch_forward<T, 64, 8>(who, *in, f.cut, out, final_state, marks, workspace, (hipStream_t)stream);
+        const auto launch = f.lanes == 4 ? launch_forward<T, 4, W> : f.lanes == 16 ? launch_forward<T, 16, W> : launch_forward<T, 64, 8>;
+        rc = launch(who, *in, f.cut, out, final_state, marks, workspace, (hipStream_t)stream);
     });
     return rc;
 }

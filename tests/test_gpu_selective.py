@@ -189,7 +189,8 @@ def test_conv_steps_are_the_sequence(m):
 SCAN_SHAPES = [  # B, D, L, N, G
     (1, 1, 1, 1, 1), (2, 3, 2, 2, 1), (1, 4, 7, 3, 2), (2, 6, 9, 16, 3), (3, 17, 40, 5, 1), (1, 8, 127, 16, 2),
     (1, 33, 128, 8, 1), (2, 20, 129, 17, 1), (1, 5, 300, 33, 1), (2, 4, 513, 4, 4), (1, 2, 1100, 16, 1), (70, 2, 3, 4, 1),
-    (1, 2, 2700, 3, 1), (2, 3, 5000, 2, 1), (260, 40, 140, 3, 1)]  # rows cut along time; two sets of channels a lane
+    (1, 2, 2700, 3, 1), (2, 3, 5000, 2, 1),  # rows cut along time
+    (260, 40, 140, 3, 1), (130, 70, 21, 3, 1), (120, 160, 33, 5, 2), (90, 256, 150, 2, 1)]  # 16 lanes a channel; 4: one tile, two, five
 
 
 def scan_case(shape, dtype, variant, seed=0):
@@ -296,8 +297,8 @@ def test_selective_scan_in_pieces_is_the_whole(m, dtype):
 
 
 def test_selective_scan_more_channels_than_a_wave_row(m):
-    """Enough channels for 16 lanes each (the forward's other form), several tiles, a group's end inside a block."""
-    for dtype, (B, D, L, N, G) in ((BF16, (4, 2100, 200, 4, 1)), (F32, (3, 2802, 131, 3, 2))):
+    """Enough channels for 16 lanes each, several tiles, a group's end inside a block; for 4 lanes each, many states."""
+    for dtype, (B, D, L, N, G) in ((BF16, (4, 2100, 200, 4, 1)), (F32, (3, 2802, 131, 3, 2)), (F16, (130, 70, 9, 250, 1))):
         a, *_ = scan_case((B, D, L, N, G), dtype, 3)
         y, final = m.fm_selective_scan(**a, return_state=True)
         ref = scan_reference(a, True)
