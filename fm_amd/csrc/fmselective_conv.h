@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256) void conv_backward_short_kernel(const T* __res
 
 // Long rows: a wave walks a row, or a segment of one, from its end to its start, a tile of 64 chunks after the other, up to
 // four in flight. What the last lane needs from behind a tile is kept from the tile before. The gradients of weight and bias
-// are summed over the whole walk in registers and across the lanes once. In bf16 70 us at (8, 4096, 2048), 5.8 TB/s; rows of
+// are summed over the whole walk in registers and across the lanes once. In bf16 72 us at (8, 4096, 2048), 5.6 TB/s; rows of
 // two tiles 88 us at (16, 4096, 1024).
 template <typename T, int W>
 __global__ __launch_bounds__(256) void conv_backward_kernel(const T* __restrict__ inputs, const T* __restrict__ out_grad,
