@@ -459,7 +459,7 @@ size_t scan_backward_lds(int N) {
 // blocks by a second kernel, always in the same order.
 // Rows that are too few to fill the GPU are cut into segments, as in forward: the first launch (ENDS) finds what each
 // segment but the first hands on of a gradient that enters it from behind.
-// Bound by vector instructions, about 29 a state and step, at two waves a SIMD (237 registers): 553 us at (8, 2048, 2048),
+// Bound by vector instructions, about 28 a state and step, at two waves a SIMD (237 registers): 553 us at (8, 2048, 2048),
 // N = 16 in bf16, the SIMDs busy for 85 % of it. What it leaves for the sums over the channels is 268 MB there.
 template <typename T, int WAVES, bool ENDS>
 __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, ScanGrads o) {
