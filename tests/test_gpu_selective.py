@@ -412,6 +412,43 @@ def test_steps_are_seen_by_a_graph_that_holds_the_states(m):
         m.fm_conv_step(rand(g, 2, 4), rand(g, 2, 4, 3), w)
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_channel_that_is_not_finite_stays_alone(m, bad):
+    """Channels side by side in a wave: the others' outputs and gradients keep their bits."""
+    g = gen(61)
+    for B, D, L in ((3, 70, 5), (2, 70, 65), (2, 9, 700)):
+        x, w, dy = rand(g, B, D, L, dtype=BF16), rand(g, D, 4), rand(g, B, D, L, dtype=BF16)
+        got = []
+        for spoiled in (False, True):
+            mine = x.clone()
+            if spoiled:
+                mine[:, 4, L // 2] = bad
+            leaves = [mine.requires_grad_(), w.detach().clone().requires_grad_()]
+            y = m.fm_conv(*leaves)
+            got.append([y, *torch.autograd.grad(y, leaves, dy)])
+        keep = [d for d in range(D) if d != 4]
+        assert not torch.isfinite(got[1][0][:, 4]).all()
+        for p, q in zip(*got):
+            axis = 1 if p.dim() == 3 else 0
+            assert torch.equal(p.index_select(axis, torch.tensor(keep, device=DEV)), q.index_select(axis, torch.tensor(keep, device=DEV)))
+    for shape in ((130, 70, 21, 3, 1), (9, 1030, 140, 2, 1), (1, 9, 700, 3, 1)):  # 4, 16, 64 lanes a channel
+        a, dy, *_ = scan_case(shape, F32, 0)
+        got = []
+        for spoiled in (False, True):
+            mine = {k: v.clone().requires_grad_() for k, v in a.items() if v is not None}
+            if spoiled:
+                with torch.no_grad():
+                    mine["tokens"][:, 4, shape[2] // 2] = bad
+            y = m.fm_selective_scan(**mine)
+            own = ("tokens", "delta", "gate", "A", "delta_bias")  # (write's and read's gradients are sums over the channels)
+            got.append([y, *torch.autograd.grad(y, [mine[k] for k in own], dy)])
+        keep = torch.tensor([d for d in range(shape[1]) if d != 4], device=DEV)
+        assert not torch.isfinite(got[1][0][:, 4]).all()
+        for p, q in zip(*got):
+            axis = 1 if p.dim() == 3 else 0
+            assert torch.equal(p.index_select(axis, keep), q.index_select(axis, keep))
+
+
 # ---- norm -------------------------------------------------------------------------------------------
 # sum of squares: at most 4 chunks of 8 in a thread and 10 levels, halved by the root; a few operations after it: c = 40
 # the row's second sum, of products: c = 80; weight's gradient: a rounding a row in a slot (8 to rows / 512), then
