@@ -102,7 +102,7 @@ def fm_norm(inputs, weight, residual=None, eps=1e-6):
         weight (D,): float32 or the inputs' dtype.
 
     Returns (out (..., D), r (..., D)): r is the residual of the next block. What the norm sees is r as it is
-    stored, rounded. Differentiable once, in inputs, weight and residual.
+    stored, rounded. Differentiable once, backwards, in inputs, weight and residual.
     """
     if _tracked(inputs, weight, residual):
         out, stream_out = FM_Norm.apply(inputs, weight, residual, eps)

@@ -12,6 +12,7 @@ implementation behind them. The reference has no counterpart of these operators.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -106,13 +107,15 @@ def _once(gradients, ctx, *grads):
 
 
 def _tracked(*tensors):
-    """Whether autograd follows a call with these arguments."""
-    if not torch.is_grad_enabled():
+    """Whether autograd follows a call with these arguments: backwards, or forwards, where a dual tensor requires no gradient
+    and the node raises (it has no forward derivative)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level < 0:  # (an attribute, where unpack_dual would cost a microsecond a tensor)
         return False
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            return True
-    return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _conv_check(inputs, weight, bias, initial_state, lengths, silu):
@@ -224,7 +227,7 @@ def fm_conv(inputs, weight, bias=None, initial_state=None, lengths=None, silu=Tr
         silu: out = s * sigmoid(s) of the sum s, else the sum itself.
         return_state: also return the last W - 1 inputs that count, the state that continues the sequence.
 
-    Returns (B, D, L), or that and the final state (B, D, W - 1). Differentiable once, in everything but lengths.
+    Returns (B, D, L), or that and the final state (B, D, W - 1). Differentiable once, backwards, in everything but lengths.
     """
     if _tracked(inputs, weight, bias, initial_state):
         out, final = FM_Conv.apply(inputs, weight, bias, initial_state, lengths, silu, return_state)
@@ -429,7 +432,8 @@ def fm_selective_scan(tokens, delta, A, write, read, skip=None, gate=None, delta
         softplus: apply it to delta + delta_bias, else the sum is dt itself.
         return_state: also return the state after the last step that counts, float32 (B, D, N).
 
-    Returns (B, D, L) of the tokens' dtype, or that and the final state. Differentiable once, in everything but lengths.
+    Returns (B, D, L) of the tokens' dtype, or that and the final state. Differentiable once, backwards, in everything but
+    lengths.
     """
     if write.dim() == 3 and read.dim() == 3:
         write, read = write.unsqueeze(1), read.unsqueeze(1)
