@@ -14,7 +14,7 @@ import torch
 
 from .. import _lib
 from .fm_scan import _ptr, _raw, _require
-from .fm_selective import _call, _dense, _gpu, _once, _parameter, _tracked, _type_of
+from .fm_selective import _call, _dense, _gpu, _not_tracked, _once, _parameter, _tracked, _type_of
 
 __all__ = ["fm_norm", "fm_norm_quantized", "FM_Norm"]
 
@@ -112,11 +112,13 @@ def fm_norm(inputs, weight, residual=None, eps=1e-6):
 
 
 def fm_norm_quantized(inputs, weight, residual=None, eps=1e-6):
-    """fm_norm with its output in 8 bits, one scale a row. Not differentiable.
+    """fm_norm with its output in 8 bits, one scale a row. Not differentiable: an argument that requires a gradient is refused
+    outside torch.no_grad().
 
     Returns (values (..., D) torch.float8_e4m3fn, scales (...) float32, r (..., D)): out is values * scales, scales are
     max |out| / 448 of each row, values are rounded to nearest even. A row of zeros, or of values below 2^-100, has scale
     0; a row with a NaN among its outputs has a NaN scale.
     """
+    _not_tracked("fm_norm_quantized", inputs, weight, residual)
     out, stream_out, _, scales, _ = _forward(inputs, weight, residual, eps, quantized=True)
     return out, scales, (inputs if residual is None else stream_out)

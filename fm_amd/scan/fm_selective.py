@@ -118,6 +118,13 @@ def _tracked(*tensors):
     return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
+def _not_tracked(call, *tensors):
+    """Refuses what a call without a derivative would detach."""
+    if _tracked(*tensors):
+        _require(False, f"{call} is not differentiable, but a tensor it was given requires a gradient or carries a tangent: "
+                        "call it under torch.no_grad(), or detach the tensor")
+
+
 def _conv_check(inputs, weight, bias, initial_state, lengths, silu):
     _gpu("inputs", inputs)
     if inputs.dim() != 3 or weight.dim() != 2:
@@ -237,7 +244,8 @@ def fm_conv(inputs, weight, bias=None, initial_state=None, lengths=None, silu=Tr
 
 
 def fm_conv_step(inputs, state, weight, bias=None, slots=None, silu=True, state_out=None):
-    """fm_conv for one token of every row; moves the state on by it. Not differentiable.
+    """fm_conv for one token of every row; moves the state on by it. Not differentiable: an argument that requires a
+    gradient is refused outside torch.no_grad().
 
     Arguments:
         inputs (B, D): channel stride 1.
@@ -264,6 +272,7 @@ def fm_conv_step(inputs, state, weight, bias=None, slots=None, silu=True, state_
         flags |= _lib.SELECTIVE_SILU
     if bias is not None:
         flags |= _parameter("bias", bias, (D,), dtype, dev, _lib.SELECTIVE_NARROW_BIAS)
+    _not_tracked("fm_conv_step", inputs, state, weight, bias, state_out)
     new = _pool(state, state_out, slots, B, D, W - 1, dtype, dev)
     S = state.shape[0]
     if slots is not None and S == 0:
@@ -447,7 +456,8 @@ def fm_selective_scan(tokens, delta, A, write, read, skip=None, gate=None, delta
 
 def fm_selective_step(tokens, state, delta, A, write, read, skip=None, gate=None, delta_bias=None, slots=None, softplus=True,
                       state_out=None):
-    """fm_selective_scan for one token of every row; moves the state on by it. Not differentiable.
+    """fm_selective_scan for one token of every row; moves the state on by it. Not differentiable: an argument that requires a
+    gradient is refused outside torch.no_grad().
 
     Arguments:
         tokens, delta, gate (B, D): channel stride 1. write, read (B, G, N) or (B, N): state stride 1.
@@ -472,6 +482,7 @@ def fm_selective_step(tokens, state, delta, A, write, read, skip=None, gate=None
     _sequence("write", write, (B, G, N), dtype, dev)
     _sequence("read", read, (B, G, N), dtype, dev)
     flags |= _slots(slots, B, dev)
+    _not_tracked("fm_selective_step", tokens, state, delta, A, write, read, skip, gate, delta_bias, state_out)
     new = _pool(state, state_out, slots, B, D, N, torch.float32, dev)
     S = state.shape[0]
     if slots is not None and S == 0:

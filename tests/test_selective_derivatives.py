@@ -60,3 +60,22 @@ def test_each_tensor_that_requires_a_gradient_makes_a_node(calls, name):
         with torch.no_grad():
             out = call(**mine)
             assert not (out[0] if isinstance(out, tuple) else out).requires_grad
+
+
+@pytest.mark.parametrize("name", ["conv_step", "step", "quantized"])
+def test_calls_without_a_derivative_refuse_what_needs_one(calls, name):
+    """As torch refuses an `out=` among tensors that require gradients."""
+    call, tensors = calls[name]
+    for k, t in tensors.items():
+        mine = {**tensors, k: t.clone().requires_grad_()}
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            call(**mine)
+        with torch.no_grad():
+            call(**mine)
+        with forward_ad.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="not differentiable"):
+            call(**{**tensors, k: forward_ad.make_dual(t, torch.ones_like(t))})
+    version = tensors["state"]._version if "state" in tensors else 0
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        call(**{k: v.clone().requires_grad_() if k in ("tokens", "inputs") else v for k, v in tensors.items()})
+    assert "state" not in tensors or tensors["state"]._version == version  # (nothing was moved on)
+    call(**tensors)
