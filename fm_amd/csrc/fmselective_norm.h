@@ -131,7 +131,8 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void norm_forward_kernel(con
         for (int k = 0; k < E; ++k) sum = __builtin_fmaf(h[j][k], h[j][k], sum);
     }
     sum = row_total<TPR>(sum, shared[0]);
-    const float inv = rsqrtf(sum / (float)D + eps);  // (also where the mean is subnormal)
+    const float mean = sum / (float)D + eps;
+    const float inv = mean == 0.0f ? 0.0f : rsqrtf(mean);  // (a row of zeros without eps is zeros; the mean may be subnormal)
     if (inv_rms && i == 0) inv_rms[row] = inv;
 #pragma unroll
     for (int j = 0; j < CH; ++j)

@@ -101,6 +101,10 @@ def fm_norm(inputs, weight, residual=None, eps=1e-6):
         inputs, residual (..., D): contiguous, one dtype; residual may be omitted (r is inputs then). D up to 16384.
         weight (D,): float32 or the inputs' dtype.
 
+    Squares are summed in float32. With eps = 0 a row whose mean square is zero there (zeros, or a root mean square below
+    2^-75) gives zeros, and nothing goes back through its norm; the same holds for a row of finite values whose sum of squares
+    is infinite there (from 2^128 on).
+
     Returns (out (..., D), r (..., D)): r is the residual of the next block. What the norm sees is r as it is
     stored, rounded. Differentiable once, backwards, in inputs, weight and residual.
     """

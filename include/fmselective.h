@@ -127,7 +127,9 @@ int fmselective_scan_step(const fmselective_scan_inputs* in, float* state_out, c
  *   r = inputs + residual (rounded to the element type, as it is stored), inv = 1 / sqrt(mean r^2 + eps)
  *   out = r inv weight
  * over `rows` dense rows of D elements, 1 <= D <= FMSELECTIVE_MAX_NORM. residual may be NULL (r is inputs, nothing
- * is stored). inv_rms (rows) float32 may be NULL; the backward call needs it. With scales (rows) float32 the output
+ * is stored). Squares are summed in float32. With eps = 0 a row whose mean square is zero there (zeros, or a root mean
+ * square below 2^-75) has inv 0 and gives zeros; so does a row of finite values whose sum is infinite (from 2^128 on).
+ * inv_rms (rows) float32 may be NULL; the backward call needs it. With scales (rows) float32 the output
  * is 8-bit e4m3 instead, one byte an element: scales = max |out| / 448 of the row, values out / scale rounded to
  * nearest even (a row of zeros, or of values below 2^-100, has scale 0 and zeros; one with a NaN among its outputs
  * has a NaN scale). */
