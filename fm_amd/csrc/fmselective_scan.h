@@ -39,6 +39,13 @@ __device__ __forceinline__ float softplus(float x) {
     return fmaxf(x, 0.0f) + l;
 }
 
+// A state's decay rate in base 2, finite where A is not or the product leaves float32: a step of length zero, such as the steps
+// behind a row's end, then leaves every state as it is (0 times infinity would be NaN), and any other forgets it at once.
+__device__ __forceinline__ float decay_rate(float A) {
+    const float r = A * kLog2E;
+    return r < -__FLT_MAX__ ? -__FLT_MAX__ : r;
+}
+
 // What the kernels need of include/fmselective.h's fmselective_scan
 struct Scan {
     const void *tokens, *delta, *gate, *write, *read, *skip, *delta_bias;
@@ -305,7 +312,7 @@ __global__ __launch_bounds__(64 * WAVES) void selective_forward_kernel(Scan p, T
                 h = __builtin_fmaf(q.x, h, q.y);
             }
         }
-        held[n] = make_float2(p.A[(int64_t)d * p.N + n] * kLog2E, h);
+        held[n] = make_float2(decay_rate(p.A[(int64_t)d * p.N + n]), h);
     }
 
     const int chunks = (p.N + NC - 1) / NC;
@@ -493,7 +500,7 @@ __global__ __launch_bounds__(64 * WAVES) void selective_backward_kernel(Scan p, 
         float e = 0.0f, rate = 0.0f;
         if (valid) {
             const int64_t at_n = row * p.N + n;
-            rate = p.A[(int64_t)d * p.N + n] * kLog2E;
+            rate = decay_rate(p.A[(int64_t)d * p.N + n]);
             if (!ENDS) {
                 if (o.final_grad) e = o.final_grad[at_n];
 #pragma unroll 4
@@ -832,7 +839,7 @@ __global__ __launch_bounds__(256) void selective_step_kernel(Step p, T* __restri
             const float dtu = dt[i] * u[i];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                h[i][k] = __builtin_fmaf(exp2_fast(dt[i] * (a[i][k] * kLog2E)), h[i][k], dtu * w[k]);
+                h[i][k] = __builtin_fmaf(exp2_fast(dt[i] * decay_rate(a[i][k])), h[i][k], dtu * w[k]);
                 y[i] = __builtin_fmaf(r[k], h[i][k], y[i]);
             }
             const int64_t d = first + 64 * i;

@@ -430,8 +430,8 @@ def fm_selective_scan(tokens, delta, A, write, read, skip=None, gate=None, delta
 
     Arguments:
         tokens, delta (B, D, L) and gate (B, D, L) or None: one dtype, time stride 1, any batch and channel stride.
-        A (D, N): float32, negative in a model whose states decay; N up to 256. Where a state grows, its growth over the
-            call's steps must be finite in float32, even while the state itself is zero.
+        A (D, N): float32, negative in a model whose states decay (minus infinity: the state forgets at once); N up to 256. Where
+            a state grows, its growth over the call's steps must be finite in float32, even while the state itself is zero.
         write, read (B, G, N, L), or (B, N, L) for one group: of the tokens' dtype, time stride 1; channel d is in
             group g = d // (D / G).
         skip, delta_bias (D,): float32 or the tokens' dtype; absent is zero.

@@ -75,7 +75,8 @@ int fmselective_conv_step(const void* inputs, int64_t batch_stride, const void* 
  * with channel d in group g = d / (D / G). tokens, delta, gate (B, D, L) and write, read (B, G, N, L) have one
  * element type and any strides but the time's, which is 1; A (D, N), states and their gradients are float32.
  * gate, skip, delta_bias, initial_state and lengths may be NULL. 1 <= N <= FMSELECTIVE_MAX_STATES, G divides D.
- * Products of decays over many steps are taken: where A is positive they must stay finite in float32. */
+ * Products of decays over many steps are taken: where A is positive they must stay finite in float32. A may be minus
+ * infinity: such a state holds the last step's term alone, and a step of length zero leaves it as it is. */
 #define FMSELECTIVE_MAX_STATES 256
 #define FMSELECTIVE_MARK 128 /* steps between the states that forward saves for backward */
 
