@@ -24,16 +24,17 @@ int check_rows(const char* who, int64_t rows, int64_t D, int dtype) {
 // (32768, 512) a wave 25 / 26, 256 threads 35 / 78; (32768, 1024) a wave 46 / 46, 256 threads 44 / 84; (16384, 1600) a wave
 // 40 / 49, 256 threads 37 / 72; (8192, 4096) a wave 50 / 68, 256 threads 46 / 51, 1024 threads 48 / 61; (4096, 8192) 256
 // threads 49 / 50, 1024 threads 46 / 55; (2048, 16384) 256 threads 50 / 76, 1024 threads 48 / 74.
-template <bool BACKWARD, typename F>
-void with_row_shape(int64_t D, int dtype, F&& f) {
-    const int64_t chunks = (D + (dtype == FMSCAN_DTYPE_F32 ? 4 : 8) - 1) / (dtype == FMSCAN_DTYPE_F32 ? 4 : 8);
+template <typename T, bool BACKWARD, typename F>
+void with_row_shape(int64_t D, F&& f) {
+    constexpr int E = fmselective::Elem<T>::E;
+    const int64_t chunks = (D + E - 1) / E;
     if (chunks <= 64) f(IntTag<64>{}, IntTag<1>{});
     else if (chunks <= 128) f(IntTag<64>{}, IntTag<2>{});
     else if (chunks <= 256) f(IntTag<BACKWARD ? 64 : 256>{}, IntTag<BACKWARD ? 4 : 1>{});
     else if (chunks <= 512) f(IntTag<256>{}, IntTag<2>{});
     else if (chunks <= 1024) f(IntTag<BACKWARD ? 256 : 1024>{}, IntTag<BACKWARD ? 4 : 1>{});
     else if (chunks <= 2048) f(IntTag<1024>{}, IntTag<2>{});
-    else f(IntTag<1024>{}, IntTag<4>{});  // FMSELECTIVE_MAX_NORM float32 values are 4096 chunks
+    else if constexpr (FMSELECTIVE_MAX_NORM / E > 2048) f(IntTag<1024>{}, IntTag<4>{});  // (float32 alone)
 }
 
 // Blocks of the backward call, each with its part of the weight's gradient: all the rows' where there are few, else as
@@ -66,11 +67,13 @@ int fmselective_norm_forward(const void* inputs, const void* residual, const voi
                               {"weight", weight, D * (flags & FMSELECTIVE_NARROW_WEIGHT ? es : 4)}}))
         return rc;
     int threads = 0;  // a row
-    with_row_shape<false>(D, dtype, [&](auto pt, auto) { threads = decltype(pt)::value; });
+    with_dtype(dtype, [&](auto tt) {
+        with_row_shape<typename decltype(tt)::type, false>(D, [&](auto pt, auto) { threads = decltype(pt)::value; });
+    });
     if (int rc = check_grid(who, (__int128)rows + 3, threads)) return rc;
     with_dtype(dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
-        with_row_shape<false>(D, dtype, [&](auto pt, auto ct) {
+        with_row_shape<T, false>(D, [&](auto pt, auto ct) {
             constexpr int TPR = decltype(pt)::value, CH = decltype(ct)::value, RPB = TPR == 64 ? 4 : 1;
             with_bool(scales != nullptr, [&](auto qt) {
                 fmselective::norm_forward_kernel<T, TPR, CH, decltype(qt)::value>
@@ -110,7 +113,7 @@ int fmselective_norm_backward(const void* out_grad, const void* residual_grad, c
     int64_t blocks = 0;
     with_dtype(dtype, [&](auto tt) {
         using T = typename decltype(tt)::type;
-        with_row_shape<true>(D, dtype, [&](auto pt, auto ct) {
+        with_row_shape<T, true>(D, [&](auto pt, auto ct) {
             constexpr int TPR = decltype(pt)::value, CH = decltype(ct)::value, RPB = TPR == 64 ? 4 : 1;
             blocks = backward_blocks(rows, RPB);
             fmselective::norm_backward_kernel<T, TPR, CH><<<(unsigned)blocks, TPR == 64 ? 256 : TPR, 0, (hipStream_t)stream>>>(
