@@ -14,7 +14,7 @@ import torch
 
 from .. import _lib
 from .fm_scan import _ptr, _raw, _require
-from .fm_selective import _call, _dense, _gpu, _not_tracked, _once, _parameter, _tracked, _type_of
+from .fm_selective import _call, _dense, _gpu, _no_derivative, _once, _parameter, _tracked, _type_of
 
 __all__ = ["fm_norm", "fm_norm_quantized", "FM_Norm"]
 
@@ -123,6 +123,7 @@ def fm_norm_quantized(inputs, weight, residual=None, eps=1e-6):
     max |out| / 448 of each row, values are rounded to nearest even. A row of zeros, or of values below 2^-100, has scale
     0; a row with a NaN among its outputs has a NaN scale.
     """
-    _not_tracked("fm_norm_quantized", inputs, weight, residual)
+    if _tracked(inputs, weight, residual):
+        _no_derivative("fm_norm_quantized")
     out, stream_out, _, scales, _ = _forward(inputs, weight, residual, eps, quantized=True)
     return out, scales, (inputs if residual is None else stream_out)

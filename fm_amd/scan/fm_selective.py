@@ -118,11 +118,10 @@ def _tracked(*tensors):
     return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
-def _not_tracked(call, *tensors):
-    """Refuses what a call without a derivative would detach."""
-    if _tracked(*tensors):
-        _require(False, f"{call} is not differentiable, but a tensor it was given requires a gradient or carries a tangent: "
-                        "call it under torch.no_grad(), or detach the tensor")
+def _no_derivative(call):
+    """For a call that autograd follows and that has no derivative: detached quietly, the gradient would be lost."""
+    _require(False, f"{call} is not differentiable, but a tensor it was given requires a gradient or carries a tangent: "
+                    "call it under torch.no_grad(), or detach the tensor")
 
 
 def _conv_check(inputs, weight, bias, initial_state, lengths, silu):
@@ -272,7 +271,8 @@ def fm_conv_step(inputs, state, weight, bias=None, slots=None, silu=True, state_
         flags |= _lib.SELECTIVE_SILU
     if bias is not None:
         flags |= _parameter("bias", bias, (D,), dtype, dev, _lib.SELECTIVE_NARROW_BIAS)
-    _not_tracked("fm_conv_step", inputs, state, weight, bias, state_out)
+    if _tracked(inputs, state, weight, bias, state_out):
+        _no_derivative("fm_conv_step")
     new = _pool(state, state_out, slots, B, D, W - 1, dtype, dev)
     S = state.shape[0]
     if slots is not None and S == 0:
@@ -482,7 +482,8 @@ def fm_selective_step(tokens, state, delta, A, write, read, skip=None, gate=None
     _sequence("write", write, (B, G, N), dtype, dev)
     _sequence("read", read, (B, G, N), dtype, dev)
     flags |= _slots(slots, B, dev)
-    _not_tracked("fm_selective_step", tokens, state, delta, A, write, read, skip, gate, delta_bias, state_out)
+    if _tracked(tokens, state, delta, A, write, read, skip, gate, delta_bias, state_out):
+        _no_derivative("fm_selective_step")
     new = _pool(state, state_out, slots, B, D, N, torch.float32, dev)
     S = state.shape[0]
     if slots is not None and S == 0:
