@@ -23,7 +23,8 @@ int check_rows(const char* who, int64_t rows, int64_t D, int dtype) {
 // barrier comes once a row instead of once a block, keeps to waves a little longer. Measured (bf16, us, forward / backward):
 // (32768, 512) a wave 25 / 26, 256 threads 35 / 78; (32768, 1024) a wave 46 / 46, 256 threads 44 / 84; (16384, 1600) a wave
 // 40 / 49, 256 threads 37 / 72; (8192, 4096) a wave 50 / 68, 256 threads 46 / 51, 1024 threads 48 / 61; (4096, 8192) 256
-// threads 49 / 50, 1024 threads 46 / 55; (2048, 16384) 256 threads 50 / 76, 1024 threads 48 / 74.
+// threads 49 / 50, 1024 threads 46 / 55; (2048, 16384) 256 threads 50 / 76, 1024 threads 48 / 74. (Backward beyond 8192
+// elements spills: 1024 threads leave a thread 128 registers, and 73 to 75 of those in 16 bits, 180 in float32, go to scratch.)
 template <typename T, bool BACKWARD, typename F>
 void with_row_shape(int64_t D, F&& f) {
     constexpr int E = fmselective::Elem<T>::E;

@@ -12,7 +12,8 @@ namespace {
 // and 7 to 8 us of 64 (512 of one), the instructions' latency; with more it is their number that counts, 3.1, 3.9 and
 // 3.5 us for each of a SIMD's waves. The fastest by that is taken: (7, 1024, 515) 57 -> 40 us with 16 lanes against 64,
 // (1, 4096, 16384) 680 -> 440 with 64 against 16, (1, 4096, 500) 26 -> 20; with 4 against 16 lanes (64, 4096, 8) 170 -> 51,
-// (32, 2048, 64) 47 -> 28, (16, 4096, 150) 91 -> 69, but (8, 4096, 200) 47 -> 52, (16, 4096, 100) 55 both.
+// (32, 2048, 64) 47 -> 28, (16, 4096, 150) 91 -> 69, but (8, 4096, 200) 47 -> 52, (16, 4096, 100) 55 both. (The rule does not
+// know N or the type: it is not measured far from N = 16, nor for float32, whose kernels hold more registers.)
 // Where 64 lanes leave less than two waves a SIMD the rows are cut, for four: (1, 1024, 16384) 225 -> 179 us,
 // (1, 512, 16384) 112 -> 95 (against a cut for two).
 constexpr int64_t kSimds = 1024;
@@ -23,8 +24,8 @@ int64_t modelled_time(int64_t tiles, int64_t waves, int64_t latency, int64_t eac
 }
 
 // A single token's call: blocks of 64 channels from which on a block takes 128 instead, two channels a lane. Measured with
-// one, two and four (bf16, N = 16, us, pools that no cache holds): (256, 4096) 46, 40, 45; (1024, 1024) 50, 42, 46;
-// (64, 4096) 15 each.
+// one, two and four (bf16, N = 16, us, four pools in turn, which no cache holds; a single one is kept by the last-level cache and
+// takes 29 with two): (256, 4096) 46, 40, 45; (1024, 1024) 50, 42, 46; (64, 4096) 15 each.
 constexpr int64_t kManyStepBlocks = 4096;
 
 struct ForwardPlan {

@@ -442,7 +442,9 @@ def fm_selective_scan(tokens, delta, A, write, read, skip=None, gate=None, delta
         return_state: also return the state after the last step that counts, float32 (B, D, N).
 
     Returns (B, D, L) of the tokens' dtype, or that and the final state. Differentiable once, backwards, in everything but
-    lengths.
+    lengths. Where a gradient is wanted the forward call keeps a state every 128 steps, B D L N / 32 bytes, and the backward call
+    holds partial sums of B D L N / 2 bytes while it runs (269 MB at (8, 2048, 2048), N = 16): more where groups are not multiples
+    of 16 channels or L not one of 128, which count as if they were.
     """
     if write.dim() == 3 and read.dim() == 3:
         write, read = write.unsqueeze(1), read.unsqueeze(1)

@@ -94,12 +94,15 @@ typedef struct fmselective_scan_inputs {
 /* Rows that are too few to fill the GPU are cut along time; what passes between the pieces goes through a workspace.
  * The forward call takes NULL (rows are then scanned in one piece, the same results up to rounding), the backward
  * call needs its own, which holds its partial sums too. Bytes that a call of these sizes can use; 0 where none or
- * where the sizes are not valid. */
+ * where the sizes are not valid.
+ * Backward's is mostly the partial sums of write's and read's gradients, 1 KiB for every 16 channels of a group, state and
+ * FMSELECTIVE_MARK steps, begun ones included: about B D L N / 2 bytes, so 269 MB at (8, 2048, 2048) with N = 16 and one group; as
+ * much for a group of one channel as for one of 16, for one step as for 128. */
 size_t fmselective_scan_workspace_bytes(int64_t B, int64_t D, int64_t L, int64_t N, int64_t G, int dtype, int backward);
 
 /* out (B, D, L); final_state (B, D, N) or NULL; marks (B, D, ceil(L / FMSELECTIVE_MARK), N) float32 or NULL: the
  * states before every FMSELECTIVE_MARK steps, which the backward call needs (those at or beyond a row's length
- * are not written). */
+ * are not specified). */
 int fmselective_scan_forward(const fmselective_scan_inputs* in, void* out, float* final_state, float* marks, void* workspace,
                              size_t workspace_bytes, void* stream);
 
