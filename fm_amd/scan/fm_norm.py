@@ -120,8 +120,9 @@ def fm_norm_quantized(inputs, weight, residual=None, eps=1e-6):
     outside torch.no_grad().
 
     Returns (values (..., D) torch.float8_e4m3fn, scales (...) float32, r (..., D)): out is values * scales, scales are
-    max |out| / 448 of each row, values are rounded to nearest even. A row of zeros, or of values below 2^-100, has scale
-    0; a row with a NaN among its outputs has a NaN scale.
+    max |out| / 448 of each row, values are out / scales in float32, rounded to nearest even (float32's own roundings decide
+    where the quotient of unrounded numbers is halfway between two values). A row of zeros, or of values below 2^-100, has
+    scale 0; a row with a NaN among its outputs has a NaN scale.
     """
     if _tracked(inputs, weight, residual):
         _no_derivative("fm_norm_quantized")
