@@ -135,8 +135,8 @@ int fmselective_scan_step(const fmselective_scan_inputs* in, float* state_out, c
  * square below 2^-75) has inv 0 and gives zeros; so does a row of finite values whose sum is infinite (from 2^128 on).
  * inv_rms (rows) float32 may be NULL; the backward call needs it. With scales (rows) float32 the output
  * is 8-bit e4m3 instead, one byte an element: scales = max |out| / 448 of the row, values out / scale, in float32, rounded
- * to nearest even: where the quotient of unrounded numbers is halfway, float32's own roundings decide (a row of zeros, or of values below 2^-100, has scale 0 and zeros; one with a NaN among its outputs
- * has a NaN scale). */
+ * to nearest even: where the quotient of unrounded numbers is halfway, float32's own roundings decide (a row of zeros, or
+ * of values below 2^-100, has scale 0 and zeros; one with a NaN among its outputs has a NaN scale). */
 #define FMSELECTIVE_MAX_NORM 16384
 int fmselective_norm_forward(const void* inputs, const void* residual, const void* weight, void* residual_out, void* out,
                              float* scales, float* inv_rms, int64_t rows, int64_t D, int dtype, unsigned flags, float eps,
