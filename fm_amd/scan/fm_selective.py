@@ -99,10 +99,19 @@ def _call(dev, entry, *args):
         _lib.check(rc)
 
 
+def _dual(tensors):
+    """Whether one of them carries a tangent of forward-mode differentiation."""
+    if forward_ad._current_level < 0:  # (an attribute, where unpack_dual would cost a microsecond a tensor)
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _once(gradients, ctx, *grads):
     """A node's gradients, differentiable once: the guard against a second time is only put up where one could follow.
     (This runs on autograd's own thread, where every Python object that the forward call has just used is in another
     core's cache: the arguments are not checked a second time either.)"""
+    if _dual(grads):
+        _require(False, "the gradient has no forward-mode derivative, but the output's gradient carries a tangent")
     return once_differentiable(gradients)(ctx, *grads) if torch.is_grad_enabled() else gradients(ctx, *grads)
 
 
@@ -113,9 +122,7 @@ def _tracked(*tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    if forward_ad._current_level < 0:  # (an attribute, where unpack_dual would cost a microsecond a tensor)
-        return False
-    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return _dual(tensors)
 
 
 def _no_derivative(call):

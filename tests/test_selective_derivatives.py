@@ -79,3 +79,18 @@ def test_calls_without_a_derivative_refuse_what_needs_one(calls, name):
         call(**{k: v.clone().requires_grad_() if k in ("tokens", "inputs") else v for k, v in tensors.items()})
     assert "state" not in tensors or tensors["state"]._version == version  # (nothing was moved on)
     call(**tensors)
+
+
+@pytest.mark.parametrize("name", SEQUENCES)
+def test_a_tangent_of_the_gradient_is_refused(calls, name):
+    """Forward over reverse: the output's gradient is the dual tensor."""
+    call, tensors = calls[name]
+    mine = {k: t.clone().requires_grad_() for k, t in tensors.items()}
+    out = call(**mine)
+    out = out[0] if isinstance(out, tuple) else out
+    dy = torch.ones_like(out)
+    torch.autograd.grad(out, list(mine.values()), dy, retain_graph=True)
+    with forward_ad.dual_level():
+        torch.autograd.grad(out, list(mine.values()), dy, retain_graph=True)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, list(mine.values()), forward_ad.make_dual(dy, torch.ones_like(dy)))
